@@ -1,0 +1,519 @@
+// Causal attention over packed sequences of different lengths on sm_100a tensor cores, forward,
+// and the schedule that its backward shares (packed.cuh has the layout of a packing).
+//
+//   o_i = sum_{j <= i + len_k - len_q} softmax_j(scale q_i . k_j) v_j   within one sequence;
+//   query head h reads kv head h / (Hq / Hkv); queries that see no key get zeros.
+//
+// One CTA per (sequence, pair of 128-query tiles, query head).  Warp 0 loads Q once and streams
+// K/V tiles by TMA, warp 1 issues the MMAs for both query tiles in turn, warps 4-7 and 8-11 are
+// the softmax of one query tile each (one row per thread, scores in TMEM, P written back over
+// them as the A operand of O += P V).  A last, partial key tile takes rows of the next sequence:
+// their probabilities are zero, but zero times an infinity or NaN of a neighbour would not be, so
+// the softmax warps clear those rows of V before the product.
+#include "attn/packed.cuh"
+#include "common/fast_exp2.cuh"
+
+#include <cmath>
+
+namespace tt {
+namespace packed {
+
+// ----------------------------------------------------------------- schedule
+constexpr int kSchedThreads = 1024;
+constexpr int kBins = 2048;  // work of an entry in tiles, clamped (order only)
+
+// Entries of sequence s, and the work of entry t (which bin: the most work first).
+__device__ __forceinline__ int entries_of(const Seq& s, int kind) {
+  const int rows = kind == kQueryPairs ? 2 * kBlock : kBlock;
+  return ((kind == kKeyTiles ? s.klen : s.qlen) + rows - 1) / rows;
+}
+__device__ __forceinline__ int bin_of(const Seq& s, bool extra, int kind, int t) {
+  const int rows = kind == kQueryPairs ? 2 * kBlock : kBlock;
+  const int work = kind == kKeyTiles ? query_tiles(s, extra, t) : key_tiles(s, extra, t * rows, rows);
+  return kBins - 1 - min(work, kBins - 1);
+}
+
+// One block: check the offsets, count entries per amount of work, and place them by falling work
+// (a counting sort; the order within one amount is arbitrary and does not reach the results).
+__global__ void __launch_bounds__(kSchedThreads) schedule_kernel(const Packing p, int kind, int2* list, int capacity,
+                                                                 int* status) {
+  __shared__ int bins[kBins];
+  __shared__ int bad, total;
+  __shared__ int warp_sum[32];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  if (tid == 0) bad = 0;
+  for (int i = tid; i < kBins; i += kSchedThreads) bins[i] = 0;
+  __syncthreads();
+  bool wrong = tid == 0 && (p.cu_q[0] != 0 || p.cu_k[0] != 0 || p.cu_q[p.B] > p.Nq || p.cu_k[p.B] > p.Nk);
+  for (int b = tid; b < p.B; b += kSchedThreads) wrong |= p.cu_q[b + 1] < p.cu_q[b] || p.cu_k[b + 1] < p.cu_k[b];
+  if (wrong) bad = 1;
+  __syncthreads();
+  if (bad) {  // nothing is computed
+    if (tid == 0) atomicCAS(status, 0, static_cast<int>(kBadIndex));
+    for (int i = tid; i < capacity; i += kSchedThreads) list[i] = make_int2(-1, 0);
+    return;
+  }
+  constexpr int kWarps = kSchedThreads / 32;
+  for (int b = warp; b <= p.B; b += kWarps) {
+    const Seq s = sequence(p, b);
+    const int n = entries_of(s, kind);
+    for (int t = lane; t < n; t += 32) atomicAdd(&bins[bin_of(s, b == p.B, kind, t)], 1);
+  }
+  __syncthreads();
+  // exclusive prefix over the bins (two per thread)
+  const int a0 = bins[2 * tid], a1 = bins[2 * tid + 1];
+  int incl = a0 + a1;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int up = __shfl_up_sync(0xffffffffu, incl, o);
+    if (lane >= o) incl += up;
+  }
+  if (lane == 31) warp_sum[warp] = incl;
+  __syncthreads();
+  int base = 0;
+  for (int w = 0; w < warp; ++w) base += warp_sum[w];
+  if (tid == kSchedThreads - 1) total = base + incl;
+  bins[2 * tid] = base + incl - a0 - a1;
+  bins[2 * tid + 1] = base + incl - a1;
+  __syncthreads();
+  for (int b = warp; b <= p.B; b += kWarps) {
+    const Seq s = sequence(p, b);
+    const int n = entries_of(s, kind);
+    for (int t = lane; t < n; t += 32) {
+      const int at = atomicAdd(&bins[bin_of(s, b == p.B, kind, t)], 1);
+      if (at < capacity) list[at] = make_int2(b, t);
+    }
+  }
+  for (int i = total + tid; i < capacity; i += kSchedThreads) list[i] = make_int2(-1, 0);
+}
+static_assert(kBins == 2 * kSchedThreads, "two bins per thread");
+
+void schedule(const Packing& p, ScheduleKind kind, int2* list, int capacity, int* status, cudaStream_t stream) {
+  schedule_kernel<<<1, kSchedThreads, 0, stream>>>(p, static_cast<int>(kind), list, capacity, status);
+  TT_CUDA_CHECK(cudaGetLastError());
+}
+
+// ----------------------------------------------------------------- forward
+constexpr int kThreads = 384;
+constexpr float kRescale = 8.0f;  // log2 units the running maximum may lag behind
+
+struct FwdParams {
+  Packing pk;
+  const int2* list;
+  int Hq, Hkv;
+  __nv_bfloat16* o;  // [Nq, Hq, D] contiguous
+  float* lse;        // [Hq, Nq] natural log (may be null)
+  float scale_log2;
+  int* status;
+};
+
+template <int D>
+struct FwdSmem {
+  static constexpr int TILE = kBlock * D * 2;
+  alignas(1024) uint8_t q[2][TILE];
+  alignas(1024) uint8_t k[2][TILE];
+  alignas(1024) uint8_t v[2][TILE];
+  uint64_t q_full;
+  uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2];
+  uint64_t s_full[2], p_full[2], o_done[2];
+  uint64_t done;
+  uint32_t tmem_slot;
+};
+
+template <int D>
+__global__ void __launch_bounds__(kThreads, 1)
+    packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
+                      const __grid_constant__ CUtensorMap tmV, const FwdParams p) {
+  static_assert(D == 64 || D == 128, "head_dim must be 64 or 128");
+  constexpr uint32_t TILE = FwdSmem<D>::TILE;
+  constexpr uint32_t IDESC_QK = idesc_bf16_f32(kBlock, kBlock, false, false);
+  constexpr uint32_t IDESC_PV = idesc_bf16_f32(kBlock, D, false, true);
+  constexpr uint32_t TMEM_COLS = 512;
+  // TMEM: S/P of tile x at columns [128 x, +128) (P: bf16 pairs in the first 64), O of tile x at 256 + x D.
+  auto S_COL = [](int x) { return static_cast<uint32_t>(x * kBlock); };
+  auto O_COL = [](int x) { return static_cast<uint32_t>(2 * kBlock + x * D); };
+
+  const int2 entry = p.list[blockIdx.x / p.Hq];
+  if (entry.x < 0) return;  // past the end of the list (uniform over the block, nothing allocated)
+  const int h = static_cast<int>(blockIdx.x) % p.Hq;
+  const int g = h / (p.Hq / p.Hkv);
+  const Seq s = sequence(p.pk, entry.x);
+  const bool extra = entry.x == p.pk.B;
+  const int i0 = entry.y * 2 * kBlock;  // first query of the pair
+  int n_x[2];
+  n_x[0] = key_tiles(s, extra, i0, kBlock);
+  n_x[1] = key_tiles(s, extra, i0 + kBlock, kBlock);
+  const int n_max = max(n_x[0], n_x[1]);
+
+  extern __shared__ uint8_t smem_raw[];
+  FwdSmem<D>& sm = *reinterpret_cast<FwdSmem<D>*>(align_ptr(smem_raw, 1024));
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  if (n_max == 0) {  // no key is seen: zeros
+    const int rows = min(2 * kBlock, s.qlen - i0);
+    constexpr int NU = D / 8;
+    for (int i = threadIdx.x; i < rows * NU; i += kThreads) {
+      const long long row = s.q0 + i0 + i / NU;
+      reinterpret_cast<uint4*>(p.o + (row * p.Hq + h) * D)[i % NU] = make_uint4(0u, 0u, 0u, 0u);
+    }
+    if (p.lse != nullptr)
+      for (int i = threadIdx.x; i < rows; i += kThreads)
+        p.lse[static_cast<long long>(h) * p.pk.Nq + s.q0 + i0 + i] = -INFINITY;
+    return;
+  }
+  // rows past the sequence in its last key tile, where it is one of those seen
+  const int n_keys = (s.klen + kBlock - 1) / kBlock;
+  const bool clean = n_max == n_keys && s.klen % kBlock != 0;
+  const int cleaner = n_x[0] == n_max ? 0 : 1;  // the tile whose P V reads the last V tile first
+
+  if (threadIdx.x == 0) {
+    tma_prefetch_desc(&tmQ);
+    tma_prefetch_desc(&tmK);
+    tma_prefetch_desc(&tmV);
+    mbar_init(&sm.q_full, 1);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&sm.k_full[i], 1);
+      mbar_init(&sm.k_empty[i], 1);
+      mbar_init(&sm.v_full[i], 1);
+      mbar_init(&sm.v_empty[i], 1);
+      mbar_init(&sm.s_full[i], 1);
+      mbar_init(&sm.p_full[i], 128);
+      mbar_init(&sm.o_done[i], 1);
+    }
+    mbar_init(&sm.done, 1);
+    fence_barrier_init();
+  }
+  if (warp == 1) {
+    tmem_alloc(&sm.tmem_slot, TMEM_COLS);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = sm.tmem_slot;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      // ------------------------------------------------ TMA producer
+      mbar_arrive_expect_tx(&sm.q_full, 2 * TILE);
+#pragma unroll
+      for (int x = 0; x < 2; ++x)
+#pragma unroll
+        for (int c = 0; c < D / 64; ++c)
+          tma_load_3d(sm.q[x] + c * kBlock * 128, &tmQ, &sm.q_full, c * 64, h, s.q0 + i0 + x * kBlock);
+      for (int j = 0; j < n_max; ++j) {
+        const int st = j & 1;
+        const uint32_t ph = (j >> 1) & 1;
+        if (!mbar_wait(&sm.k_empty[st], ph ^ 1u, p.status, kTimeoutEmpty)) break;
+        mbar_arrive_expect_tx(&sm.k_full[st], TILE);
+#pragma unroll
+        for (int c = 0; c < D / 64; ++c)
+          tma_load_3d(sm.k[st] + c * kBlock * 128, &tmK, &sm.k_full[st], c * 64, g, s.k0 + j * kBlock);
+        if (!mbar_wait(&sm.v_empty[st], ph ^ 1u, p.status, kTimeoutEmpty)) break;
+        mbar_arrive_expect_tx(&sm.v_full[st], TILE);
+#pragma unroll
+        for (int c = 0; c < D / 64; ++c)
+          tma_load_3d(sm.v[st] + c * kBlock * 128, &tmV, &sm.v_full[st], c * 64, g, s.k0 + j * kBlock);
+      }
+      mbar_wait(&sm.q_full, 0, p.status, kTimeoutOther);
+      for (int j = max(0, n_max - 2); j < n_max; ++j) {  // every copy has landed before the block ends
+        mbar_wait(&sm.k_full[j & 1], (j >> 1) & 1, p.status, kTimeoutOther);
+        mbar_wait(&sm.v_full[j & 1], (j >> 1) & 1, p.status, kTimeoutOther);
+      }
+    }
+  } else if (warp == 1) {
+    if (lane == 0) {
+      // ------------------------------------------------ MMA issuer, the two query tiles in turn
+      auto qk = [&](int x, int j) {
+        const uint32_t q_base = smem_u32(sm.q[x]);
+        const uint32_t k_base = smem_u32(sm.k[j & 1]);
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk) {
+          const uint32_t off = (kk >> 2) * (kBlock * 128) + (kk & 3) * 32;
+          umma_f16_ss(tmem + S_COL(x), sdesc_sw128(q_base + off, 16, 1024), sdesc_sw128(k_base + off, 16, 1024),
+                      IDESC_QK, kk > 0 ? 1u : 0u);
+        }
+        umma_commit(&sm.s_full[x]);
+      };
+      auto pv = [&](int x, int j) {
+        const uint32_t v_base = smem_u32(sm.v[j & 1]);
+#pragma unroll
+        for (int kk = 0; kk < kBlock / 16; ++kk)
+          umma_f16_ts(tmem + O_COL(x), tmem + S_COL(x) + kk * 8, sdesc_sw128(v_base + kk * 2048, kBlock * 128, 1024),
+                      IDESC_PV, (j > 0 || kk > 0) ? 1u : 0u);
+        umma_commit(&sm.o_done[x]);
+      };
+      bool ok = mbar_wait(&sm.q_full, 0, p.status, kTimeoutFull) && mbar_wait(&sm.k_full[0], 0, p.status, kTimeoutFull);
+      if (ok) {
+        tc_fence_after();
+        for (int x = 0; x < 2; ++x)
+          if (n_x[x] > 0) qk(x, 0);
+        umma_commit(&sm.k_empty[0]);
+      }
+      for (int j = 0; ok && j < n_max; ++j) {
+        const bool next = j + 1 < n_max;
+        if (!mbar_wait(&sm.v_full[j & 1], (j >> 1) & 1, p.status, kTimeoutFull)) break;
+        if (next && !mbar_wait(&sm.k_full[(j + 1) & 1], ((j + 1) >> 1) & 1, p.status, kTimeoutFull)) break;
+        tc_fence_after();
+        for (int x = 0; x < 2; ++x) {
+          if (j < n_x[x]) {
+            if (!mbar_wait(&sm.p_full[x], j & 1, p.status, kTimeoutFull)) {
+              ok = false;
+              break;
+            }
+            tc_fence_after();
+            pv(x, j);
+          }
+          if (j + 1 < n_x[x]) qk(x, j + 1);  // in order after PV(x, j), which read P from these columns
+        }
+        if (!ok) break;
+        umma_commit(&sm.v_empty[j & 1]);
+        if (next) umma_commit(&sm.k_empty[(j + 1) & 1]);
+      }
+      umma_commit(&sm.done);
+      mbar_wait(&sm.done, 0, p.status, kTimeoutOther);
+    }
+  } else if (warp >= 4) {
+    // ------------------------------------------------ softmax warpgroups: x = 0 (warps 4-7), 1 (warps 8-11)
+    const int x = (warp - 4) >> 2;
+    const int quarter = warp & 3;
+    const int r = quarter * 32 + lane;
+    const int qi = i0 + x * kBlock + r;  // query within the sequence
+    const uint32_t lane_addr = static_cast<uint32_t>(quarter * 32) << 16;
+    const uint32_t s_addr = tmem + lane_addr + S_COL(x);
+    const uint32_t o_addr = tmem + lane_addr + O_COL(x);
+    const int lim = min(qi + s.off, s.klen - 1);  // last key this row sees (negative: none)
+    const int n = n_x[x];
+    const float sl2 = p.scale_log2;
+    float m_ref = -INFINITY;  // reference maximum, scaled log2 units
+    float l = 0.0f;
+    bool ok = true;
+    for (int j = 0; j < n; ++j) {
+      if (!mbar_wait_warp(&sm.s_full[x], j & 1, p.status, kTimeoutAccFull)) {
+        ok = false;
+        break;
+      }
+      tc_fence_after();
+      const int key0 = j * kBlock;
+      const bool need_mask = key0 + kBlock - 1 > lim;
+      // Scores in four chunks of 32 columns, each chunk's TMEM load under the previous one's math.
+      // The reference maximum rises only when a chunk's maximum exceeds it by more than 2^8, so no
+      // exponential overflows; what was computed under an older reference is rescaled after.
+      const float m_start = m_ref;
+      float cref[4], csum[4];
+      {
+        uint32_t bufA[32], bufB[32];
+        tmem_ld32(s_addr, bufA);
+        tmem_ld_wait();
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          uint32_t(&cur)[32] = (c & 1) ? bufB : bufA;
+          uint32_t(&nxt)[32] = (c & 1) ? bufA : bufB;
+          if (c < 3) tmem_ld32(s_addr + (c + 1) * 32, nxt);
+          float v[32];
+#pragma unroll
+          for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(cur[i]);
+          if (need_mask) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) v[i] = key0 + c * 32 + i > lim ? -INFINITY : v[i];
+          }
+          float e[32];
+          float mq[4];
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            float m = fmax3(v[q], v[q + 4], v[q + 8]);
+            m = fmax3(m, v[q + 12], v[q + 16]);
+            m = fmax3(m, v[q + 20], v[q + 24]);
+            mq[q] = fmaxf(m, v[q + 28]);
+          }
+          const float mcs = fmax3(mq[0], mq[1], fmaxf(mq[2], mq[3])) * sl2;
+          if (mcs > m_ref + kRescale) m_ref = mcs;  // also the first visible chunk (m_ref = -inf)
+          const float neg_m = (m_ref == -INFINITY) ? 0.0f : -m_ref;
+          const unsigned long long s2 = f2_pack(sl2, sl2), nm2 = f2_pack(neg_m, neg_m);
+#pragma unroll
+          for (int i = 0; i < 32; i += 2) {
+            const unsigned long long r2 = f2_fma(f2_pack(v[i], v[i + 1]), s2, nm2);
+            f2_unpack(r2, e[i], e[i + 1]);
+          }
+          // two of eight exponentials on the FMA pipe, so that MUFU does not bound the tile
+#pragma unroll
+          for (int i = 0; i < 32; i += 2) {
+            if ((i & 7) == 6) {
+              exp2_poly2(e[i], e[i + 1]);
+            } else {
+              e[i] = ex2_mufu(e[i]);
+              e[i + 1] = ex2_mufu(e[i + 1]);
+            }
+          }
+          unsigned long long sa = f2_pack(e[0], e[1]), sb = f2_pack(e[2], e[3]);
+#pragma unroll
+          for (int i = 4; i < 32; i += 4) {
+            sa = f2_add(sa, f2_pack(e[i], e[i + 1]));
+            sb = f2_add(sb, f2_pack(e[i + 2], e[i + 3]));
+          }
+          float a0, a1;
+          f2_unpack(f2_add(sa, sb), a0, a1);
+          csum[c] = a0 + a1;
+          cref[c] = m_ref;
+          uint32_t pk[16];
+#pragma unroll
+          for (int i = 0; i < 16; ++i) pk[i] = pack_bf16x2(e[2 * i], e[2 * i + 1]);
+          tmem_st16(s_addr + c * 16, pk);
+          if (c < 3) tmem_ld_wait();
+        }
+      }
+      float rs = 0.0f;
+      float cf[4];
+      bool fix = false;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        cf[c] = (cref[c] == m_ref) ? 1.0f : ex2_mufu(cref[c] - m_ref);
+        fix |= cf[c] != 1.0f;
+        rs = fmaf(csum[c], cf[c], rs);
+      }
+      if (__any_sync(0xffffffffu, fix)) {  // rare: P chunks under an older reference
+        tmem_st_wait();
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          uint32_t pv[16];
+          tmem_ld16(s_addr + c * 16, pv);
+          tmem_ld_wait();
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const float2 f = unpack_bf16x2(pv[i]);
+            pv[i] = pack_bf16x2(f.x * cf[c], f.y * cf[c]);
+          }
+          tmem_st16(s_addr + c * 16, pv);
+        }
+      }
+      const float alpha = (m_start == m_ref) ? 1.0f : ex2_mufu(m_start - m_ref);
+      l = l * alpha + rs;
+      if (__any_sync(0xffffffffu, j > 0 && alpha != 1.0f)) {  // rare: O under an older reference
+#pragma unroll
+        for (int c = 0; c < D; c += 16) {
+          uint32_t ov[16];
+          tmem_ld16(o_addr + c, ov);
+          tmem_ld_wait();
+#pragma unroll
+          for (int i = 0; i < 16; ++i) ov[i] = __float_as_uint(__uint_as_float(ov[i]) * alpha);
+          tmem_st16(o_addr + c, ov);
+        }
+      }
+      // S(j) is there, so P V(j - 2) is done and this buffer's current or last phase is V(j)'s
+      if (clean && x == cleaner && j == n_max - 1) {
+        if (!mbar_wait_warp(&sm.v_full[j & 1], (j >> 1) & 1, p.status, kTimeoutFull)) {
+          ok = false;
+          break;
+        }
+        clear_rows<D>(sm.v[j & 1], s.klen - key0, r, kBlock);
+        fence_proxy_async();
+      }
+      tmem_st_wait();
+      tc_fence_before();
+      mbar_arrive(&sm.p_full[x]);
+    }
+    // ------------------------------------------------ O / l and the log-sum-exp
+    const bool row_ok = qi < s.qlen;
+    const long long row = s.q0 + qi;
+    __nv_bfloat16* orow = p.o + (row * p.Hq + h) * D;
+    if (n == 0) {
+      if (row_ok) {
+#pragma unroll
+        for (int c = 0; c < D / 8; ++c) reinterpret_cast<uint4*>(orow)[c] = make_uint4(0u, 0u, 0u, 0u);
+        if (p.lse != nullptr) p.lse[static_cast<long long>(h) * p.pk.Nq + row] = -INFINITY;
+      }
+    } else if (ok && mbar_wait_warp(&sm.o_done[x], (n - 1) & 1, p.status, kTimeoutAccFull)) {
+      tc_fence_after();
+      const bool seen = lim >= 0;
+      const float inv_l = 1.0f / l;
+#pragma unroll
+      for (int c = 0; c < D; c += 32) {
+        uint32_t ov[32];
+        tmem_ld32(o_addr + c, ov);
+        tmem_ld_wait();
+        if (row_ok) {
+          uint4* dst = reinterpret_cast<uint4*>(orow + c);
+          float f[32];
+#pragma unroll
+          for (int i = 0; i < 32; ++i) f[i] = seen ? __uint_as_float(ov[i]) * inv_l : 0.0f;
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            dst[i] = make_uint4(pack_bf16x2(f[8 * i], f[8 * i + 1]), pack_bf16x2(f[8 * i + 2], f[8 * i + 3]),
+                                pack_bf16x2(f[8 * i + 4], f[8 * i + 5]), pack_bf16x2(f[8 * i + 6], f[8 * i + 7]));
+        }
+      }
+      if (row_ok && p.lse != nullptr)
+        p.lse[static_cast<long long>(h) * p.pk.Nq + row] = seen ? (m_ref + log2f(l)) * 0.69314718055994531f : -INFINITY;
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 1) tmem_dealloc(tmem, TMEM_COLS);
+}
+
+}  // namespace packed
+
+// int32 elements of the schedule that packed_attn_fwd needs.
+int64_t packed_attn_schedule_numel(int64_t Nq, int64_t Nk, int64_t B) {
+  using namespace packed;
+  return 2 * std::max(max_tiles(Nq, B, kBlock), max_tiles(Nk, B, kBlock));
+}
+
+// q [Nq, Hq, D], k/v [Nk, Hkv, D] bf16 (any 16-byte-aligned strides), cu_q/cu_k int32 [B + 1] ->
+// o [Nq, Hq, D] contiguous, lse fp32 [Hq, Nq] (optional).  sched: int32 scratch.
+void packed_attn_fwd(torch::Tensor q, torch::Tensor k, torch::Tensor v, torch::Tensor cu_q, torch::Tensor cu_k,
+                     double scale, torch::Tensor o, c10::optional<torch::Tensor> lse, torch::Tensor sched) {
+  using namespace packed;
+  TT_CHECK(q.dim() == 3 && k.dim() == 3, "packed_attn: q and k must be [tokens, heads, D]");
+  const int64_t Nq = q.size(0), Hq = q.size(1), D = q.size(2), Nk = k.size(0), Hkv = k.size(1);
+  TT_CHECK(D == 64 || D == 128, "packed_attn: head_dim must be 64 or 128");
+  TT_CHECK(Hkv >= 1 && Hq >= 1 && Hq % Hkv == 0, "packed_attn: Hq must be a multiple of Hkv");
+  check_heads(q, Hq, D, "packed_attn q");
+  check_heads(k, Hkv, D, "packed_attn k");
+  check_heads(v, Hkv, D, "packed_attn v");
+  TT_CHECK(v.size(0) == Nk, "packed_attn: k and v must have as many tokens");
+  check_offsets(cu_q, -1, "cu_seqlens");
+  check_offsets(cu_k, cu_q.numel(), "cu_seqlens_k");
+  const int64_t B = cu_q.numel() - 1;
+  check_cuda_bf16(o, "o");
+  TT_CHECK(o.is_contiguous() && o.numel() == Nq * Hq * D && reinterpret_cast<uintptr_t>(o.data_ptr()) % 16 == 0,
+           "packed_attn: o must be contiguous [Nq, Hq, D]");
+  if (lse.has_value())
+    TT_CHECK(lse->scalar_type() == torch::kFloat32 && lse->is_contiguous() && lse->numel() == Hq * Nq, "packed_attn: lse must be fp32 [Hq, Nq]");
+  TT_CHECK(scale > 0 && std::isfinite(scale), "packed_attn: scale must be positive and finite");
+  TT_CHECK(sched.scalar_type() == torch::kInt32 && sched.is_contiguous() && sched.numel() >= packed_attn_schedule_numel(Nq, Nk, B) &&
+               reinterpret_cast<uintptr_t>(sched.data_ptr()) % 8 == 0,
+           "packed_attn: schedule scratch too small");
+  if (Nq == 0) return;
+  const c10::cuda::CUDAGuard guard(q.device());
+  TT_CUDA_CHECK(cudaSetDevice(q.get_device()));  // binds the context to this thread: the tensor maps need one
+  if (Nk == 0) {  // no keys at all (a tensor map cannot be empty)
+    o.zero_();
+    if (lse.has_value()) lse->fill_(-INFINITY);
+    return;
+  }
+  FwdParams p{};
+  p.pk = packing_of(q, k, cu_q, cu_k);
+  p.list = reinterpret_cast<const int2*>(sched.data_ptr<int>());
+  p.Hq = static_cast<int>(Hq);
+  p.Hkv = static_cast<int>(Hkv);
+  p.o = reinterpret_cast<__nv_bfloat16*>(o.data_ptr());
+  p.lse = lse.has_value() ? lse->data_ptr<float>() : nullptr;
+  p.scale_log2 = static_cast<float>(scale * 1.4426950408889634);
+  p.status = device_status_ptr(q.get_device());
+  const CUtensorMap tq = head_map_3d(q, kBlock, "q"), tk = head_map_3d(k, kBlock, "k"), tv = head_map_3d(v, kBlock, "v");
+  const int64_t entries = max_tiles(Nq, B, 2 * kBlock);
+  TT_CHECK(entries * Hq < (1LL << 31), "packed_attn: too many tiles");
+  schedule(p.pk, kQueryPairs, reinterpret_cast<int2*>(sched.data_ptr<int>()), static_cast<int>(entries), p.status, cur_stream());
+  auto launch = [&](auto kern, size_t smem) {
+    TT_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
+    kern<<<static_cast<unsigned>(entries * Hq), kThreads, smem, cur_stream()>>>(tq, tk, tv, p);
+  };
+  if (D == 128) launch(packed_fwd_kernel<128>, sizeof(FwdSmem<128>) + 1024);
+  else launch(packed_fwd_kernel<64>, sizeof(FwdSmem<64>) + 1024);
+  TT_CUDA_CHECK(cudaGetLastError());
+}
+
+}  // namespace tt

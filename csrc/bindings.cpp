@@ -78,6 +78,29 @@ void decode_advance(torch::Tensor nxt, torch::Tensor tokens, int64_t P, torch::T
 void decode_attention(torch::Tensor q, torch::Tensor k_pages, torch::Tensor v_pages, torch::Tensor page_table,
                       c10::optional<torch::Tensor> len_dev, int64_t len_host, int64_t splits, double scale,
                       torch::Tensor o_part, torch::Tensor ml_part, torch::Tensor out);
+void token_stats_fwd(torch::Tensor logits, torch::Tensor targets, int64_t k, int64_t ignore_index, torch::Tensor lp,
+                     torch::Tensor ent, torch::Tensor ms, torch::Tensor top_lp, torch::Tensor top_id);
+void token_stats_bwd(torch::Tensor logits, torch::Tensor targets, int64_t k, int64_t ignore_index, torch::Tensor ent,
+                     torch::Tensor ms, torch::Tensor top_id, c10::optional<torch::Tensor> g_lp,
+                     c10::optional<torch::Tensor> g_ent, c10::optional<torch::Tensor> g_top, torch::Tensor grad);
+void rotary_append(torch::Tensor qkv, torch::Tensor cos_t, torch::Tensor sin_t, int64_t Hq, int64_t Hkv, int64_t D,
+                   torch::Tensor cu, c10::optional<torch::Tensor> start, bool inverse, torch::Tensor q_out,
+                   c10::optional<torch::Tensor> k_out, c10::optional<torch::Tensor> k_pages,
+                   c10::optional<torch::Tensor> v_pages, c10::optional<torch::Tensor> page_table);
+void fork_pages(torch::Tensor k_pages, torch::Tensor v_pages, torch::Tensor page_table, torch::Tensor seq_lens,
+                torch::Tensor parents, torch::Tensor children, torch::Tensor fresh);
+void move_pages(torch::Tensor k_pages, torch::Tensor v_pages, torch::Tensor page_table, torch::Tensor src,
+                torch::Tensor dst);
+std::vector<int64_t> paged_attention_workspace(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t max_keys, int64_t device);
+void paged_attention(torch::Tensor q, torch::Tensor k_pages, torch::Tensor v_pages, torch::Tensor page_table,
+                     torch::Tensor seq_lens, double scale, torch::Tensor part, torch::Tensor counters, torch::Tensor out);
+int64_t packed_attn_schedule_numel(int64_t Nq, int64_t Nk, int64_t B);
+void packed_attn_fwd(torch::Tensor q, torch::Tensor k, torch::Tensor v, torch::Tensor cu_q, torch::Tensor cu_k,
+                     double scale, torch::Tensor o, c10::optional<torch::Tensor> lse, torch::Tensor sched);
+int64_t packed_attn_stats_numel(int64_t Nq, int64_t Hq, int64_t B);
+void packed_attn_bwd(torch::Tensor q, torch::Tensor k, torch::Tensor v, torch::Tensor o, torch::Tensor dout,
+                     torch::Tensor lse, torch::Tensor cu_q, torch::Tensor cu_k, double scale, torch::Tensor dq,
+                     torch::Tensor dk, torch::Tensor dv, torch::Tensor stats, torch::Tensor sched);
 void ep_allgather_counts(int64_t gid, torch::Tensor counts, int64_t dst_off);
 void ep_scatter(int64_t gid, torch::Tensor x, int64_t k, torch::Tensor tgt, torch::Tensor dst, int64_t recv_off,
                 int64_t cap, c10::optional<torch::Tensor> w, c10::optional<torch::Tensor> y_pairs,
@@ -241,6 +264,20 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("lp_all") = py::none());
   m.def("decode_num_splits", checked("decode_num_splits", &tt::decode_num_splits), "split-KV CTAs per (sequence, kv head) for a max length");
   m.def("decode_attention", checked("decode_attention", &tt::decode_attention), "split-KV paged decode attention (GQA-native) + combine");
+  m.def("token_stats_fwd", checked("token_stats_fwd", &tt::token_stats_fwd),
+        "log-probs of given tokens, entropy and top-k alternatives of logits rows");
+  m.def("token_stats_bwd", checked("token_stats_bwd", &tt::token_stats_bwd), "gradient of token_stats_fwd w.r.t. the logits");
+  m.def("rotary_append", checked("rotary_append", &tt::rotary_append),
+        "RoPE of packed tokens by their position in their sequence, and append of k/v to the sequences' pages");
+  m.def("fork_pages", checked("fork_pages", &tt::fork_pages), "children share their parent's full pages and copy its last one");
+  m.def("move_pages", checked("move_pages", &tt::move_pages), "move pages of every layer and rewrite the page table");
+  m.def("paged_attention_workspace", &tt::paged_attention_workspace, "(fp32, int32) elements paged_attention needs");
+  m.def("paged_attention", checked("paged_attention", &tt::paged_attention),
+        "attention of one new token per sequence over pages, a length per sequence");
+  m.def("packed_attn_schedule_numel", &tt::packed_attn_schedule_numel);
+  m.def("packed_attn_fwd", checked("packed_attn_fwd", &tt::packed_attn_fwd), "causal attention over packed sequences (tcgen05)");
+  m.def("packed_attn_stats_numel", &tt::packed_attn_stats_numel);
+  m.def("packed_attn_bwd", checked("packed_attn_bwd", &tt::packed_attn_bwd), "backward of packed_attn_fwd (tcgen05, fixed order of sums)");
   m.def("ep_allgather_counts", checked("ep_allgather_counts", &tt::ep_allgather_counts), "EP: all-gather per-expert counts into the heap");
   m.def("ep_scatter", checked("ep_scatter", &tt::ep_scatter), "EP dispatch: pair rows to their owners' receive buffers (peer stores)",
         py::arg("gid"), py::arg("x"), py::arg("k"), py::arg("tgt"), py::arg("dst"), py::arg("recv_off"),

@@ -27,9 +27,14 @@ SOURCES = [
     "fused/norm.cu",
     "fused/elementwise.cu",
     "fused/sample.cu",
+    "fused/token_stats.cu",
     "attn/attn_fwd.cu",
     "attn/attn_bwd.cu",
     "attn/decode.cu",
+    "attn/packed_fwd.cu",
+    "attn/packed_bwd.cu",
+    "attn/paged_decode.cu",
+    "cache/pages.cu",
     "moe/moe.cu",
     "moe/ep.cu",
 ]
