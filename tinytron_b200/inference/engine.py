@@ -171,6 +171,21 @@ class InferenceEngine:
         return PagedKVCache.contiguous(self.model_config, batch_size, self.device, self.dtype, max_seq_len=max_seq_len)
 
     # ------------------------------------------------------------------ generation
+    def generate_ragged(self, prompts, max_new_tokens: int, num_samples: int = 1, temperature: float = 1.0, top_k=None,
+                        top_p=None, eos_token_id: int | None = None, alternatives: int = 0, cache=None):
+        """Continuations of prompts of different lengths (a list of 1-D token tensors), ``num_samples`` of each.
+
+        The prompts are prefilled packed in one pass; the samples of a prompt share its full cache pages; decode runs
+        one captured step for all of them, and a sequence that has drawn ``eos_token_id`` attends to nothing from
+        then on.  Returns a :class:`~tinytron_b200.inference.ragged.RaggedGeneration` with the tokens, the log-prob
+        each was drawn with, the model's own log-prob and entropy, and ``alternatives`` top tokens per step.
+        ``cache``: a :class:`~tinytron_b200.inference.ragged.RaggedKVCache` to work in (default: one of the right
+        size for this call); the sequences are freed again.  SEP size must be 1."""
+        from .ragged import generate_ragged
+
+        return generate_ragged(self, prompts, max_new_tokens, num_samples, temperature, top_k, top_p, eos_token_id,
+                               alternatives, cache)
+
     @torch.no_grad()
     def generate(self, input_ids: torch.Tensor, max_new_tokens: int, temperature: float = 1.0, top_k=None,
                  top_p=None, eos_token_id: int | None = None, return_stats: bool = False,

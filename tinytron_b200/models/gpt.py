@@ -164,6 +164,41 @@ class GPT(nn.Module):
         return ops.lm_head_token_logprobs(h, self.lm_head.weight, targets, self.loss_fn.ignore_index).view(
             targets.shape)
 
+    def packed_token_stats(self, idx, targets, cu_seqlens, top_k: int = 0, max_seqlen: int | None = None,
+                           temperature: float = 1.0):
+        """Statistics (:class:`~tinytron_b200.ops.TokenStats`, differentiable) of ``targets`` [N] under the model's
+        next-token distributions over sequences packed end to end: ``idx`` [N], ``cu_seqlens`` int32 [S + 1].
+        Targets equal to the ignore index (-100) are not scored."""
+        x = ops.embedding(idx, self.wte.weight)
+        pending = None
+        for blk in self.blocks:
+            x, h = ops.add_rmsnorm(x, pending, blk.ln_1.weight, self.eps)
+            a = blk.attn.forward_packed(h, cu_seqlens, max_seqlen)
+            x, h = ops.add_rmsnorm(x, a, blk.ln_2.weight, self.eps)
+            out = blk.mlp(h.unsqueeze(0))
+            pending = (out[0] if self.use_moe else out).squeeze(0)
+        _, h = ops.add_rmsnorm(x, pending, self.lnf.weight, self.eps)
+        logits = ops.linear(h, self.lm_head.weight)
+        if temperature != 1.0:
+            logits = logits / temperature
+        return ops.token_stats(logits, targets, top_k, self.loss_fn.ignore_index)
+
+    def forward_ragged(self, idx, step, rows=None):
+        """Logits [N, V] (of ``rows`` only, if given) of the tokens ``idx`` [N] of one
+        :class:`~tinytron_b200.inference.ragged.RaggedStep`; their keys and values are appended to its cache."""
+        x = ops.embedding(idx, self.wte.weight)
+        pending = None
+        for blk in self.blocks:
+            x, h = ops.add_rmsnorm(x, pending, blk.ln_1.weight, self.eps)
+            a = blk.attn.forward_ragged(h, step)
+            x, h = ops.add_rmsnorm(x, a, blk.ln_2.weight, self.eps)
+            out = blk.mlp(h.unsqueeze(0), use_cache=True)
+            pending = (out[0] if self.use_moe else out).squeeze(0)
+        if rows is not None:
+            x, pending = x[rows], pending[rows]
+        _, h = ops.add_rmsnorm(x, pending, self.lnf.weight, self.eps)
+        return ops.lm_logits(h, self.lm_head.weight)
+
     def _trunk(self, idx, targets, position_offset: int = 0, aux_stats: list | None = None):
         """Embedding -> blocks -> final norm; returns (normalised hidden states, MoE aux loss).
         With ``aux_stats`` (a list) the MoE layers append their local load-balancing

@@ -122,6 +122,37 @@ class Attention(nn.Module):
         y = gather_heads_from_ranks(o, B, T, Hq, hd, sp, sp_group)
         return ops.linear(y, self.c_proj.weight)
 
+    # ------------------------------------------------------------------ ragged
+    def forward_packed(self, h: torch.Tensor, cu_seqlens: torch.Tensor, max_seqlen: int | None = None) -> torch.Tensor:
+        """h [N, D], sequences of different lengths packed end to end (positions restart at each)."""
+        Hq, Hkv, hd = self.num_attention_heads, self.num_key_value_heads, self.head_dim
+        if sp_context()[1] > 1:
+            raise ValueError("packed sequences do not run sequence parallel (SP size must be 1)")
+        qkv = ops.linear(h, self.q_proj.weight, self.k_proj.weight, self.v_proj.weight)
+        o = ops.rotary_packed_attention(qkv, cu_seqlens, Hq, Hkv, hd, self.rope_theta, max_seqlen)
+        return ops.linear(o, self.c_proj.weight)
+
+    def forward_ragged(self, h: torch.Tensor, step) -> torch.Tensor:
+        """h [N, D], the tokens of one :class:`~tinytron_b200.inference.ragged.RaggedStep`: rotated and appended to
+        their sequences' pages; whole prompts attend to each other, single tokens to their pages."""
+        from tinytron_b200.ops.rope import rope_tables
+
+        Hq, Hkv, hd = self.num_attention_heads, self.num_key_value_heads, self.head_dim
+        n = h.shape[0]
+        cache = step.cache
+        qkv = ops.linear(h, self.q_proj.weight, self.k_proj.weight, self.v_proj.weight)
+        cos, sin = rope_tables(hd, self.rope_theta, cache.max_seq_len, h.device)
+        kp, vp = cache.k_pages[self.layer_idx], cache.v_pages[self.layer_idx]
+        decode = step.seq_lens is not None
+        q, k = ops.rotary_append(qkv, cos, sin, Hq, Hkv, step.cu_seqlens, step.start, kp, vp, step.page_table,
+                                 want_k=not decode)
+        if decode:
+            o = ops.paged_attention(q, kp, vp, step.page_table, step.seq_lens, workspace=cache.workspace(n, Hq))
+        else:
+            v = qkv.view(n, Hq + 2 * Hkv, hd)[:, Hq + Hkv:]
+            o = ops.packed_attention(q, k, v, step.cu_seqlens)
+        return ops.linear(o.reshape(n, Hq * hd), self.c_proj.weight)
+
     # ------------------------------------------------------------------ generic / cached
     def forward(self, x: torch.Tensor, past_kv=None, use_cache: bool = False, position_offset: int = 0):
         if not use_cache and past_kv is None:

@@ -11,8 +11,9 @@ import math
 import torch
 import torch.nn.functional as F
 
-from .ragged import (PagedAttentionWorkspace, TokenStats, fork_pages, move_pages, packed_attention,  # noqa: F401
-                     paged_attention, paged_attention_workspace, rotary_append, rotary_packed_attention, token_stats)
+from .ragged import (IGNORE_INDEX, PagedAttentionWorkspace, TokenStats, fork_pages, move_pages,  # noqa: F401
+                     packed_attention, paged_attention, paged_attention_workspace, rotary_append,
+                     rotary_packed_attention, token_stats)
 from .rope import rope_reference
 
 

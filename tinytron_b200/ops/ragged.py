@@ -443,7 +443,7 @@ def _token_stats_cpu(logits, targets, top_k, ignore_index):
     y = torch.log_softmax(torch.where(scored[:, None], logits.float(), zero), -1)
     lp = torch.where(scored, y.gather(1, t[:, None])[:, 0], zero)
     p = y.exp()
-    ent = torch.where(scored, -torch.where(p > 0, p * y, zero).sum(-1), zero)
+    ent = torch.where(scored, -(p * torch.where(p > 0, y, zero)).sum(-1), zero)  # p log p is 0 where p is
     ids = torch.sort(y.detach(), dim=-1, descending=True, stable=True).indices[:, :top_k]
     top = torch.where(scored[:, None], y.gather(1, ids), zero)
     return lp, ent, top, torch.where(scored[:, None], ids, torch.full_like(ids, -1))
