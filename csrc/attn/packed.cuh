@@ -74,6 +74,68 @@ __device__ __forceinline__ void clear_rows(uint8_t* tile, int from, int t, int t
       *reinterpret_cast<uint4*>(tile + c * kBlock * 128 + from * 128 + i * 16) = make_uint4(0u, 0u, 0u, 0u);
 }
 
+// ----------------------------------------------------------------- products
+// A product's descriptors live in uniform registers.  Issued by one lane of a diverged warp they are put together
+// there anew for every instruction (measured: about 130 cycles an instruction that the tensor core does in 64); so
+// the whole warp walks the issue loop, addresses are warp-uniform sums of precomputed low words, and only the
+// elected lane runs the instructions themselves.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t e;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(e));
+  return e != 0;
+}
+// Descriptor words (see sdesc_sw128): 8-row groups 1024 bytes apart, 128-byte swizzle.
+constexpr uint32_t kDescHi = (1024u >> 4) | (1u << 14) | (2u << 29);
+__device__ __forceinline__ uint32_t desc_k_major(const void* tile) { return (smem_u32(tile) >> 4) | (1u << 16); }
+__device__ __forceinline__ uint32_t desc_mn_major(const void* tile) {  // 64-element chunks 128 rows of 128 bytes apart
+  return (smem_u32(tile) >> 4) | (((kBlock * 128u) >> 4) << 16);
+}
+__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a_lo, uint32_t b_lo, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\tsetp.ne.b32 p, %5, 0;\n\tmov.b64 a, {%1, %3};\n\tmov.b64 b, {%2, %3};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %4, p;\n\t}" ::"r"(d),
+      "r"(a_lo), "r"(b_lo), "r"(kDescHi), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a_tmem, uint32_t b_lo, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b64 b;\n\tsetp.ne.b32 p, %5, 0;\n\tmov.b64 b, {%2, %3};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %4, p;\n\t}" ::"r"(d),
+      "r"(a_tmem), "r"(b_lo), "r"(kDescHi), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// d [128 x 128] = A B^T over D, both tiles [128 rows x D] K-major; `done` follows it.
+template <int D>
+__device__ __forceinline__ void product_abt(bool lead, uint32_t d, uint32_t a_lo, uint32_t b_lo, uint64_t* done) {
+  constexpr uint32_t kIdesc = idesc_bf16_f32(kBlock, kBlock, false, false);
+  if (lead) {
+#pragma unroll
+    for (int kk = 0; kk < D / 16; ++kk) {
+      const uint32_t off = ((kk >> 2) * (kBlock * 128) + (kk & 3) * 32) >> 4;
+      mma_ss(d, a_lo + off, b_lo + off, kIdesc, kk > 0 ? 1u : 0u);
+    }
+    umma_commit(done);
+  }
+  __syncwarp();
+}
+// d [128 x D] (+)= A B: A [128 x 128] as bf16 pairs in TMEM, `kGroup` of its columns in each `kGroup` 32-bit columns (the
+// first half of them), B [128 rows x D] in shared memory.
+template <int D, int kGroup>
+__device__ __forceinline__ void product_ab(bool lead, uint32_t d, uint32_t a_tmem, uint32_t b_lo, bool accumulate) {
+  constexpr uint32_t kIdesc = idesc_bf16_f32(kBlock, D, false, true);
+  const uint32_t first = accumulate ? 1u : 0u;
+  if (lead) {
+#pragma unroll
+    for (int kk = 0; kk < kBlock / 16; ++kk)
+      mma_ts(d, a_tmem + kk * 16 / kGroup * kGroup + (kk * 16 % kGroup) / 2, b_lo + kk * (2048 >> 4), kIdesc, kk > 0 ? 1u : first);
+  }
+  __syncwarp();
+}
+__device__ __forceinline__ void commit(bool lead, uint64_t* bar) {
+  if (lead) umma_commit(bar);
+  __syncwarp();
+}
+
 // 3-D tensor map of bf16 [tokens, heads, D] (strides in elements), box {64, 1, rows}, 128-byte swizzle.
 inline CUtensorMap head_map_3d(const torch::Tensor& t, int rows, const char* name) {
   const std::string n(name);

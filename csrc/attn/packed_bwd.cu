@@ -27,40 +27,61 @@
 namespace tt {
 namespace packed {
 
-constexpr int kBwdThreads = 384;  // warp 0 TMA, warp 1 MMA, warps 4..11 two compute warpgroups
-constexpr int kHalf = kBlock / 2;
+constexpr int kGroups = 4;               // compute warpgroups, 32 score columns each
+constexpr int kCols = kBlock / kGroups;  // 32
+constexpr int kBwdThreads = 128 + kGroups * 128;  // warp 0 TMA, warp 1 MMA, warps 4..19 compute
+constexpr uint32_t kComputeThreads = kGroups * 128;
+// Registers per thread after setmaxnreg: the launch gives 640 threads 96 each, the first warpgroup (TMA and MMA
+// issue) hands 32 of its own to the four compute warpgroups, 8 each.
+constexpr int kRegIssue = 64, kRegCompute = 104;
+static_assert(kRegIssue + kGroups * kRegCompute <= (1 + kGroups) * 96, "register split exceeds the launch");
 
-// Probabilities of 64 scores: 2^(s scale_log2 - l2), two of eight on the FMA pipe.
-template <bool kPerColumn>
-__device__ __forceinline__ void probabilities(const uint32_t (&raw)[kHalf], float (&pv)[kHalf], float scale_log2,
-                                              const float* l2, float l2_row) {
+__device__ __forceinline__ unsigned long long f2_mul(unsigned long long a, unsigned long long b) {
+  unsigned long long d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+
+// Probabilities of 32 scores in pairs: 2^(s scale_log2 + add), add = -lse2 of the column (or row).
+template <typename Add>
+__device__ __forceinline__ void probabilities(const uint32_t (&raw)[kCols], unsigned long long (&pv)[kCols / 2],
+                                              float scale_log2, Add add) {
   const unsigned long long s2 = f2_pack(scale_log2, scale_log2);
 #pragma unroll
-  for (int i = 0; i < kHalf; i += 2) {
+  for (int i = 0; i < kCols / 2; ++i) {
     float a, b;
-    const unsigned long long sub = kPerColumn ? f2_pack(-l2[i], -l2[i + 1]) : f2_pack(-l2_row, -l2_row);
-    f2_unpack(f2_fma(f2_pack(__uint_as_float(raw[i]), __uint_as_float(raw[i + 1])), s2, sub), a, b);
-    if ((i & 7) == 6) {
-      exp2_poly2(a, b);
-    } else {
-      a = ex2_mufu(a);
-      b = ex2_mufu(b);
-    }
-    pv[i] = a;
-    pv[i + 1] = b;
+    f2_unpack(f2_fma(f2_pack(__uint_as_float(raw[2 * i]), __uint_as_float(raw[2 * i + 1])), s2, add(i)), a, b);
+    pv[i] = f2_pack(ex2_mufu(a), ex2_mufu(b));
+  }
+}
+__device__ __forceinline__ uint32_t pack_pair(unsigned long long v) {
+  float a, b;
+  f2_unpack(v, a, b);
+  return pack_bf16x2(a, b);
+}
+// Pairs of columns [lo, hi) kept, the others zero.
+__device__ __forceinline__ void keep_columns(unsigned long long (&v)[kCols / 2], int lo, int hi) {
+#pragma unroll
+  for (int i = 0; i < kCols / 2; ++i) {
+    float a, b;
+    f2_unpack(v[i], a, b);
+    v[i] = f2_pack((2 * i >= lo && 2 * i < hi) ? a : 0.0f, (2 * i + 1 >= lo && 2 * i + 1 < hi) ? b : 0.0f);
   }
 }
 
 // ----------------------------------------------------------------- statistics per query row
-// lse2[h][r] = lse log2e and delta[h][r] = dO . O in tile-aligned rows (packed.cuh: pad_row0); rows past a
-// sequence and rows that see no key get +inf and 0 (probability 0).  One block per 128-row slot.
+// Addends of the row's scores and dP: neg_lse2[h][r] = -lse log2e and neg_delta[h][r] = -dO . O in tile-aligned rows
+// (packed.cuh: pad_row0); rows past a sequence and rows that see no key get -inf and 0 (probability 0).  kStatsRows
+// rows of a 128-row slot per block: the 16-byte loads of a row are few, so the parallelism has to come from the rows.
+constexpr int kStatsRows = 16;
 __global__ void __launch_bounds__(256) packed_stats_kernel(const Packing p, const int2* __restrict__ list,
                                                            const __nv_bfloat16* __restrict__ o,
                                                            const __nv_bfloat16* __restrict__ dout,
-                                                           const float* __restrict__ lse, float* __restrict__ lse2,
-                                                           float* __restrict__ delta, long long pad_rows, int Hq, int D) {
+                                                           const float* __restrict__ lse, float* __restrict__ neg_lse2,
+                                                           float* __restrict__ neg_delta, long long pad_rows, int Hq, int D) {
   if (list[0].x < 0) return;  // the schedule found the offsets unusable
-  const int slot = blockIdx.x;
+  const int slot = blockIdx.x / (kBlock / kStatsRows);
+  const int r0 = blockIdx.x % (kBlock / kStatsRows) * kStatsRows;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   // the sequence whose slots include this one: the last b with cu_q[b] / 128 + b <= slot
   int b = 0, n = p.B + 1;
@@ -76,13 +97,13 @@ __global__ void __launch_bounds__(256) packed_stats_kernel(const Packing p, cons
   const Seq s = sequence(p, b);
   const int i0 = slot * kBlock - s.pad_row0;  // first query of this slot
   const int vecs = Hq * D / 8, per_head = D / 8;
-  for (int r = warp; r < kBlock; r += 8) {
+  for (int r = r0 + warp; r < r0 + kStatsRows; r += 8) {
     const int qi = i0 + r;
     const long long out = static_cast<long long>(slot) * kBlock + r;
     if (qi >= s.qlen || qi + s.off < 0 || b == p.B) {
       for (int h = lane; h < Hq; h += 32) {
-        lse2[h * pad_rows + out] = INFINITY;
-        delta[h * pad_rows + out] = 0.0f;
+        neg_lse2[h * pad_rows + out] = -INFINITY;
+        neg_delta[h * pad_rows + out] = 0.0f;
       }
       continue;
     }
@@ -106,8 +127,8 @@ __global__ void __launch_bounds__(256) packed_stats_kernel(const Packing p, cons
       for (int off = per_head / 2; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
       if (i < vecs && (i & (per_head - 1)) == 0) {
         const int h = i / per_head;
-        delta[h * pad_rows + out] = sum;
-        lse2[h * pad_rows + out] = lse[static_cast<long long>(h) * p.Nq + tok] * 1.4426950408889634f;
+        neg_delta[h * pad_rows + out] = -sum;
+        neg_lse2[h * pad_rows + out] = lse[static_cast<long long>(h) * p.Nq + tok] * -1.4426950408889634f;
       }
     }
   }
@@ -117,8 +138,8 @@ struct BwdParams {
   Packing pk;
   const int2* list;
   int Hq, Hkv;
-  const float* lse2;   // [Hq, pad_rows]
-  const float* delta;  // [Hq, pad_rows]
+  const float* neg_lse2;   // [Hq, pad_rows]
+  const float* neg_delta;  // [Hq, pad_rows]
   long long pad_rows;
   __nv_bfloat16* d0;   // dq, or dk
   __nv_bfloat16* d1;   // dv
@@ -127,24 +148,19 @@ struct BwdParams {
   int* status;
 };
 
-// 64 accumulator columns-halves of a row, scaled, as bf16.
+// W accumulator columns of a row (16 or 32), scaled, as bf16.
 template <int W>
 __device__ __forceinline__ void store_row(uint32_t taddr, __nv_bfloat16* dst, float scale, bool row_ok) {
+  uint32_t rr[W];
+  if constexpr (W == 32) tmem_ld32(taddr, rr);
+  else tmem_ld16(taddr, rr);
+  tmem_ld_wait();
+  if (row_ok) {
+    uint32_t w[W / 2];
 #pragma unroll
-  for (int c = 0; c < W; c += 32) {
-    uint32_t rr[32];
-    tmem_ld32(taddr + c, rr);
-    tmem_ld_wait();
-    if (row_ok) {
-      float f[32];
+    for (int i = 0; i < W / 2; ++i) w[i] = pack_bf16x2(__uint_as_float(rr[2 * i]) * scale, __uint_as_float(rr[2 * i + 1]) * scale);
 #pragma unroll
-      for (int i = 0; i < 32; ++i) f[i] = __uint_as_float(rr[i]) * scale;
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        reinterpret_cast<uint4*>(dst + c)[i] =
-            make_uint4(pack_bf16x2(f[8 * i], f[8 * i + 1]), pack_bf16x2(f[8 * i + 2], f[8 * i + 3]),
-                       pack_bf16x2(f[8 * i + 4], f[8 * i + 5]), pack_bf16x2(f[8 * i + 6], f[8 * i + 7]));
-    }
+    for (int i = 0; i < W / 8; ++i) reinterpret_cast<uint4*>(dst)[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
   }
 }
 
@@ -156,8 +172,8 @@ struct DkvSmem {
   alignas(1024) uint8_t v[TILE];
   alignas(1024) uint8_t q[2][TILE];
   alignas(1024) uint8_t dout[2][TILE];
-  alignas(16) float lse2[2][kBlock];
-  alignas(16) float delta[2][kBlock];
+  alignas(16) float neg_lse2[2][kBlock];
+  alignas(16) float neg_delta[2][kBlock];
   uint64_t kv_full, qdo_full[2], qdo_empty[2], s_full, p_ready, dp_full, ds_ready, done;
   uint32_t tmem_slot;
 };
@@ -166,15 +182,13 @@ struct DkvSmem {
 //   S^T(0), dP^T(0); per it: [p_ready] dV += P^T dO, S^T(it + 1); [ds_ready] dK += dS^T Q, dP^T(it + 1)
 // Compute: P(0); per it: dS(it), P(it + 1).  So dS is formed while the tensor core runs dV and the next
 // scores, and the next exponentials while it runs dK and the next dP.
-// P^T (dS^T) of a warpgroup's 64 queries is written over the columns that the same warpgroup read
-// its scores (dP) from, so the two warpgroups need not wait for each other.
+// P^T (dS^T) of a warpgroup's 32 queries is written over the columns that the same warpgroup read
+// its scores (dP) from, so the warpgroups need not wait for each other.
 template <int D>
 __global__ void __launch_bounds__(kBwdThreads, 1)
     packed_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                       const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmDO, const BwdParams p) {
   constexpr uint32_t TILE = DkvSmem<D>::TILE;
-  constexpr uint32_t ID_S = idesc_bf16_f32(kBlock, kBlock, false, false);  // S^T, dP^T
-  constexpr uint32_t ID_G = idesc_bf16_f32(kBlock, D, false, true);        // dV, dK (A from TMEM)
   constexpr uint32_t S_COL = 0, DP_COL = kBlock, DV_COL = 2 * kBlock, DK_COL = 2 * kBlock + D;
   constexpr uint32_t TMEM_COLS = 512;
   const int2 entry = p.list[blockIdx.x / p.Hkv];
@@ -213,9 +227,9 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       mbar_init(&sm.qdo_empty[i], 1);
     }
     mbar_init(&sm.s_full, 1);
-    mbar_init(&sm.p_ready, 256);
+    mbar_init(&sm.p_ready, kComputeThreads);
     mbar_init(&sm.dp_full, 1);
-    mbar_init(&sm.ds_ready, 256);
+    mbar_init(&sm.ds_ready, kComputeThreads);
     mbar_init(&sm.done, 1);
     fence_barrier_init();
   }
@@ -229,6 +243,8 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
   const uint32_t tmem = sm.tmem_slot;
   const int last_qt = (s.qlen + kBlock - 1) / kBlock - 1;
 
+  if (warp < 4) {
+  setmaxnreg_dec<kRegIssue>();
   if (warp == 0) {
     if (lane == 0) {
       // ------------------------------------------------ producer (Q, dO, statistics double-buffered)
@@ -250,103 +266,80 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
           tma_load_3d(sm.dout[st] + c * kBlock * 128, &tmDO, &sm.qdo_full[st], c * 64, h, s.q0 + qt * kBlock);
         }
         const long long vo = h * p.pad_rows + s.pad_row0 + static_cast<long long>(qt) * kBlock;
-        bulk_load_1d(sm.lse2[st], p.lse2 + vo, kBlock * 4, &sm.qdo_full[st]);
-        bulk_load_1d(sm.delta[st], p.delta + vo, kBlock * 4, &sm.qdo_full[st]);
+        bulk_load_1d(sm.neg_lse2[st], p.neg_lse2 + vo, kBlock * 4, &sm.qdo_full[st]);
+        bulk_load_1d(sm.neg_delta[st], p.neg_delta + vo, kBlock * 4, &sm.qdo_full[st]);
       }
       mbar_wait(&sm.kv_full, 0, p.status, kTimeoutOther);
       for (int it = max(0, n_iter - 2); it < n_iter; ++it)
         mbar_wait(&sm.qdo_full[it & 1], (it >> 1) & 1, p.status, kTimeoutOther);
     }
   } else if (warp == 1) {
-    if (lane == 0) {
-      // ------------------------------------------------ MMA issuer
-      const uint32_t k_b = smem_u32(sm.k), v_b = smem_u32(sm.v);
-      auto scores = [&](uint32_t col, uint32_t a_b, uint32_t b_b, uint64_t* bar) {  // [128 keys x 128 queries]
-#pragma unroll
-        for (int kk = 0; kk < D / 16; ++kk) {
-          const uint32_t off = (kk >> 2) * (kBlock * 128) + (kk & 3) * 32;
-          umma_f16_ss(tmem + col, sdesc_sw128(a_b + off, 16, 1024), sdesc_sw128(b_b + off, 16, 1024), ID_S, kk > 0 ? 1u : 0u);
-        }
-        umma_commit(bar);
-      };
-      auto grads = [&](uint32_t acc, uint32_t a_col, uint32_t b_b, bool first) {  // [128 keys x D] += A [keys x queries] B
-#pragma unroll
-        for (int kk = 0; kk < kBlock / 16; ++kk)
-          umma_f16_ts(tmem + acc, tmem + a_col + (kk >> 2) * kHalf + (kk & 3) * 8,
-                      sdesc_sw128(b_b + kk * 2048, kBlock * 128, 1024), ID_G, (!first || kk > 0) ? 1u : 0u);
-      };
-      bool ok = mbar_wait(&sm.kv_full, 0, p.status, kTimeoutFull) && mbar_wait(&sm.qdo_full[0], 0, p.status, kTimeoutFull);
-      if (ok) {
-        tc_fence_after();
-        scores(S_COL, k_b, smem_u32(sm.q[0]), &sm.s_full);
-        scores(DP_COL, v_b, smem_u32(sm.dout[0]), &sm.dp_full);
-      }
-      for (int it = 0; ok && it < n_iter; ++it) {
-        const uint32_t ph = it & 1;
-        const bool next = it + 1 < n_iter;
-        if (!mbar_wait(&sm.p_ready, ph, p.status, kTimeoutFull)) break;
-        tc_fence_after();
-        grads(DV_COL, S_COL, smem_u32(sm.dout[it & 1]), it == 0);
-        if (next) {  // in order after dV, which reads P^T from the same columns
-          if (!mbar_wait(&sm.qdo_full[(it + 1) & 1], ((it + 1) >> 1) & 1, p.status, kTimeoutFull)) break;
-          tc_fence_after();
-          scores(S_COL, k_b, smem_u32(sm.q[(it + 1) & 1]), &sm.s_full);
-        }
-        if (!mbar_wait(&sm.ds_ready, ph, p.status, kTimeoutFull)) break;
-        tc_fence_after();
-        grads(DK_COL, DP_COL, smem_u32(sm.q[it & 1]), it == 0);
-        umma_commit(&sm.qdo_empty[it & 1]);
-        if (next) scores(DP_COL, v_b, smem_u32(sm.dout[(it + 1) & 1]), &sm.dp_full);
-      }
-      umma_commit(&sm.done);
-      mbar_wait(&sm.done, 0, p.status, kTimeoutOther);
+    // ------------------------------------------------ MMA issuer
+    const bool lead = elect_one();
+    const uint32_t k_lo = desc_k_major(sm.k), v_lo = desc_k_major(sm.v);
+    auto score = [&](int it) { product_abt<D>(lead, tmem + S_COL, k_lo, desc_k_major(sm.q[it & 1]), &sm.s_full); };
+    auto dprob = [&](int it) { product_abt<D>(lead, tmem + DP_COL, v_lo, desc_k_major(sm.dout[it & 1]), &sm.dp_full); };
+    bool ok = mbar_wait_warp(&sm.kv_full, 0, p.status, kTimeoutFull) && mbar_wait_warp(&sm.qdo_full[0], 0, p.status, kTimeoutFull);
+    if (ok) {
+      tc_fence_after();
+      score(0);
+      dprob(0);
     }
-  } else if (warp >= 4) {
-    // ------------------------------------------------ compute warpgroups: 64 queries each, one key per thread
-    const int half = (warp - 4) >> 2;
+    for (int it = 0; ok && it < n_iter; ++it) {
+      const uint32_t ph = it & 1;
+      const bool next = it + 1 < n_iter;
+      if (!mbar_wait_warp(&sm.p_ready, ph, p.status, kTimeoutFull)) break;
+      tc_fence_after();
+      product_ab<D, kCols>(lead, tmem + DV_COL, tmem + S_COL, desc_mn_major(sm.dout[it & 1]), it > 0);
+      if (next) {  // in order after dV, which reads P^T from the same columns
+        if (!mbar_wait_warp(&sm.qdo_full[(it + 1) & 1], ((it + 1) >> 1) & 1, p.status, kTimeoutFull)) break;
+        tc_fence_after();
+        score(it + 1);
+      }
+      if (!mbar_wait_warp(&sm.ds_ready, ph, p.status, kTimeoutFull)) break;
+      tc_fence_after();
+      product_ab<D, kCols>(lead, tmem + DK_COL, tmem + DP_COL, desc_mn_major(sm.q[it & 1]), it > 0);
+      commit(lead, &sm.qdo_empty[it & 1]);
+      if (next) dprob(it + 1);
+    }
+    commit(lead, &sm.done);
+    mbar_wait_warp(&sm.done, 0, p.status, kTimeoutOther);
+  }
+  } else {
+    setmaxnreg_inc<kRegCompute>();
+    // ------------------------------------------------ compute warpgroups: 32 queries each, one key per thread
+    const int wg = (warp - 4) >> 2;
     const int quarter = warp & 3;
     const int r = quarter * 32 + lane;
     const uint32_t lane_addr = static_cast<uint32_t>(quarter * 32) << 16;
-    const uint32_t s_addr = tmem + lane_addr + S_COL + half * kHalf;
-    const uint32_t dp_addr = tmem + lane_addr + DP_COL + half * kHalf;
+    const uint32_t s_addr = tmem + lane_addr + S_COL + wg * kCols;
+    const uint32_t dp_addr = tmem + lane_addr + DP_COL + wg * kCols;
     const int key = j0 + r;
-    float pv[kHalf];
-    // queries [lo, hi) of this warpgroup's 64 see the key
-    auto bounds = [&](int it, int& lo, int& hi) {
-      const int c0 = (qt0 + it % per_head) * kBlock + half * kHalf;
-      lo = key - s.off - c0;
-      hi = s.qlen - c0;
-    };
-    auto p_phase = [&](int it) -> bool {
+    const int key_row = key - s.off - wg * kCols;  // minus a query tile's first query: first column that sees the key
+    const int end_row = s.qlen - wg * kCols;       // likewise: columns that are queries of the sequence
+    unsigned long long pv[kCols / 2];
+    auto p_phase = [&](int it, int qt) -> bool {
       const int buf = it & 1;
       if (!mbar_wait_warp(&sm.s_full, it & 1, p.status, kTimeoutAccFull)) return false;
       if (!mbar_wait_warp(&sm.qdo_full[buf], (it >> 1) & 1, p.status, kTimeoutFull)) return false;  // the statistics
       tc_fence_after();
-      uint32_t raw[kHalf];
-      tmem_ld32(s_addr, *reinterpret_cast<uint32_t(*)[32]>(&raw[0]));
-      tmem_ld32(s_addr + 32, *reinterpret_cast<uint32_t(*)[32]>(&raw[32]));
+      uint32_t raw[kCols];
+      tmem_ld32(s_addr, raw);
+      const ulonglong2* nl = reinterpret_cast<const ulonglong2*>(sm.neg_lse2[buf] + wg * kCols);
       tmem_ld_wait();
-      probabilities<true>(raw, pv, p.scale_log2, sm.lse2[buf] + half * kHalf, 0.0f);
-      int lo, hi;
-      bounds(it, lo, hi);
-      if (lo > 0 || hi < kHalf) {
+      probabilities(raw, pv, p.scale_log2, [&](int i) { return (i & 1) ? nl[i >> 1].y : nl[i >> 1].x; });
+      const int lo = key_row - qt * kBlock, hi = end_row - qt * kBlock;
+      if (lo > 0 || hi < kCols) keep_columns(pv, lo, hi);
+      uint32_t pk[16];
 #pragma unroll
-        for (int i = 0; i < kHalf; ++i) pv[i] = (i >= lo && i < hi) ? pv[i] : 0.0f;
-      }
-#pragma unroll
-      for (int c = 0; c < kHalf; c += 32) {
-        uint32_t pk[16];
-#pragma unroll
-        for (int i = 0; i < 16; ++i) pk[i] = pack_bf16x2(pv[c + 2 * i], pv[c + 2 * i + 1]);
-        tmem_st16(s_addr + (c >> 1), pk);
-      }
-      const int qt = qt0 + it % per_head;
+      for (int i = 0; i < 16; ++i) pk[i] = pack_pair(pv[i]);
+      tmem_st16(s_addr, pk);
       if (qt == last_qt && s.qlen % kBlock != 0) {
         // The tile ends inside: once dP(it), the last product to read these rows as they are, is done, clear
         // dO's and Q's rows of the next sequence.
         if (!mbar_wait_warp(&sm.dp_full, it & 1, p.status, kTimeoutAccFull)) return false;
-        clear_rows<D>(sm.dout[buf], s.qlen - qt * kBlock, threadIdx.x - 128, 256);
-        clear_rows<D>(sm.q[buf], s.qlen - qt * kBlock, threadIdx.x - 128, 256);
+        clear_rows<D>(sm.dout[buf], s.qlen - qt * kBlock, threadIdx.x - 128, kComputeThreads);
+        clear_rows<D>(sm.q[buf], s.qlen - qt * kBlock, threadIdx.x - 128, kComputeThreads);
         fence_proxy_async();
       }
       tmem_st_wait();
@@ -354,7 +347,8 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       mbar_arrive(&sm.p_ready);
       return true;
     };
-    bool ok = p_phase(0);
+    int qt = qt0;  // query tile of iteration it (its head is it / per_head)
+    bool ok = p_phase(0, qt);
     for (int it = 0; ok && it < n_iter; ++it) {
       const int buf = it & 1;
       // ---- dS^T = P^T (dP^T - delta), the scale goes to the end
@@ -364,43 +358,34 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       }
       tc_fence_after();
       {
-        int lo, hi;
-        bounds(it, lo, hi);
-        const bool masked = lo > 0 || hi < kHalf;
-        const float* dl = sm.delta[buf] + half * kHalf;
-        uint32_t d0[32], d1[32];
-        tmem_ld32(dp_addr, d0);
-        tmem_ld32(dp_addr + 32, d1);
+        const ulonglong2* nd = reinterpret_cast<const ulonglong2*>(sm.neg_delta[buf] + wg * kCols);
+        uint32_t d[kCols];
+        tmem_ld32(dp_addr, d);
         tmem_ld_wait();
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          const uint32_t(&cur)[32] = c ? d1 : d0;
-          float ds[32];
+        for (int i = 0; i < kCols / 2; ++i)
+          pv[i] = f2_mul(pv[i], f2_add(f2_pack(__uint_as_float(d[2 * i]), __uint_as_float(d[2 * i + 1])), (i & 1) ? nd[i >> 1].y : nd[i >> 1].x));
+        const int lo = key_row - qt * kBlock, hi = end_row - qt * kBlock;
+        if (lo > 0 || hi < kCols) keep_columns(pv, lo, hi);
+        uint32_t pk[16];
 #pragma unroll
-          for (int i = 0; i < 32; ++i) ds[i] = pv[c * 32 + i] * (__uint_as_float(cur[i]) - dl[c * 32 + i]);
-          if (masked) {
-#pragma unroll
-            for (int i = 0; i < 32; ++i) ds[i] = (c * 32 + i >= lo && c * 32 + i < hi) ? ds[i] : 0.0f;
-          }
-          uint32_t pk[16];
-#pragma unroll
-          for (int i = 0; i < 16; ++i) pk[i] = pack_bf16x2(ds[2 * i], ds[2 * i + 1]);
-          tmem_st16(dp_addr + c * 16, pk);
-        }
+        for (int i = 0; i < 16; ++i) pk[i] = pack_pair(pv[i]);
+        tmem_st16(dp_addr, pk);
       }
       tmem_st_wait();
       tc_fence_before();
       mbar_arrive(&sm.ds_ready);
-      if (it + 1 < n_iter && !p_phase(it + 1)) ok = false;
+      if (++qt > last_qt) qt = qt0;
+      if (it + 1 < n_iter && !p_phase(it + 1, qt)) ok = false;
     }
-    // ---- dK, dV of this thread's key, half of the head dim per warpgroup
+    // ---- dK, dV of this thread's key, a quarter of the head dim per warpgroup
     if (ok && mbar_wait_warp(&sm.done, 0, p.status, kTimeoutAccFull)) {
       tc_fence_after();
       const bool key_ok = key < s.klen;
       const long long row = s.k0 + key;
-      constexpr int DH = D / 2;
-      store_row<DH>(tmem + lane_addr + DK_COL + half * DH, p.d0 + row * p.d0_n + g * p.d0_h + half * DH, p.scale, key_ok);
-      store_row<DH>(tmem + lane_addr + DV_COL + half * DH, p.d1 + row * p.d1_n + g * p.d1_h + half * DH, 1.0f, key_ok);
+      constexpr int W = D / kGroups;
+      store_row<W>(tmem + lane_addr + DK_COL + wg * W, p.d0 + row * p.d0_n + g * p.d0_h + wg * W, p.scale, key_ok);
+      store_row<W>(tmem + lane_addr + DV_COL + wg * W, p.d1 + row * p.d1_n + g * p.d1_h + wg * W, 1.0f, key_ok);
     }
   }
   tc_fence_before();
@@ -435,8 +420,6 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     packed_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                      const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmDO, const BwdParams p) {
   constexpr uint32_t TILE = DqSmem<D>::TILE;
-  constexpr uint32_t ID_S = idesc_bf16_f32(kBlock, kBlock, false, false);
-  constexpr uint32_t ID_G = idesc_bf16_f32(kBlock, D, false, true);
   constexpr uint32_t DP_COL = 2 * kBlock, DQ_COL = 3 * kBlock;
   constexpr uint32_t TMEM_COLS = 512;
   const int2 entry = p.list[blockIdx.x / p.Hq];
@@ -475,8 +458,8 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       mbar_init(&sm.s_full[i], 1);
     }
     mbar_init(&sm.dp_full, 1);
-    mbar_init(&sm.dp_taken, 256);
-    mbar_init(&sm.ds_ready, 256);
+    mbar_init(&sm.dp_taken, kComputeThreads);
+    mbar_init(&sm.ds_ready, kComputeThreads);
     mbar_init(&sm.done, 1);
     fence_barrier_init();
   }
@@ -516,119 +499,97 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       for (int j = max(0, n - 2); j < n; ++j) mbar_wait(&sm.v_full[j & 1], (j >> 1) & 1, p.status, kTimeoutOther);
     }
   } else if (warp == 1) {
-    if (lane == 0) {
-      // ------------------------------------------------ MMA issuer
-      const uint32_t q_b = smem_u32(sm.q), do_b = smem_u32(sm.dout);
-      auto scores = [&](uint32_t col, uint32_t a_b, uint32_t b_b, uint64_t* bar) {  // [128 queries x 128 keys]
-#pragma unroll
-        for (int kk = 0; kk < D / 16; ++kk) {
-          const uint32_t off = (kk >> 2) * (kBlock * 128) + (kk & 3) * 32;
-          umma_f16_ss(tmem + col, sdesc_sw128(a_b + off, 16, 1024), sdesc_sw128(b_b + off, 16, 1024), ID_S, kk > 0 ? 1u : 0u);
-        }
-        umma_commit(bar);
-      };
-      auto score = [&](int j) { scores((j & 1) * kBlock, q_b, smem_u32(sm.k[j % 3]), &sm.s_full[j & 1]); };
-      auto dprob = [&](int j) {
-        scores(DP_COL, do_b, smem_u32(sm.v[j & 1]), &sm.dp_full);
-        umma_commit(&sm.v_empty[j & 1]);
-      };
-      bool ok = mbar_wait(&sm.q_full, 0, p.status, kTimeoutFull) && mbar_wait(&sm.k_full[0], 0, p.status, kTimeoutFull);
-      if (ok) {
-        tc_fence_after();
-        score(0);
-        ok = mbar_wait(&sm.v_full[0], 0, p.status, kTimeoutFull);
-      }
-      if (ok) {
-        tc_fence_after();
-        dprob(0);
-        if (n > 1) {
-          ok = mbar_wait(&sm.k_full[1], 0, p.status, kTimeoutFull);
-          if (ok) {
-            tc_fence_after();
-            score(1);
-          }
-        }
-      }
-      for (int j = 0; ok && j < n; ++j) {
-        if (j + 1 < n) {
-          if (!mbar_wait(&sm.v_full[(j + 1) & 1], ((j + 1) >> 1) & 1, p.status, kTimeoutFull)) break;
-          if (!mbar_wait(&sm.dp_taken, j & 1, p.status, kTimeoutFull)) break;
-          tc_fence_after();
-          dprob(j + 1);
-        }
-        if (!mbar_wait(&sm.ds_ready, j & 1, p.status, kTimeoutFull)) break;
-        tc_fence_after();
-        const uint32_t k_b = smem_u32(sm.k[j % 3]);
-#pragma unroll
-        for (int kk = 0; kk < kBlock / 16; ++kk)
-          umma_f16_ts(tmem + DQ_COL, tmem + (j & 1) * kBlock + (kk >> 2) * kHalf + (kk & 3) * 8,
-                      sdesc_sw128(k_b + kk * 2048, kBlock * 128, 1024), ID_G, (j > 0 || kk > 0) ? 1u : 0u);
-        umma_commit(&sm.k_empty[j % 3]);
-        if (j + 2 < n) {  // in order after dQ(j), which reads dS from the same columns
-          if (!mbar_wait(&sm.k_full[(j + 2) % 3], ((j + 2) / 3) & 1, p.status, kTimeoutFull)) break;
-          tc_fence_after();
-          score(j + 2);
-        }
-      }
-      umma_commit(&sm.done);
-      mbar_wait(&sm.done, 0, p.status, kTimeoutOther);
+    // ------------------------------------------------ MMA issuer
+    const bool lead = elect_one();
+    const uint32_t q_lo = desc_k_major(sm.q), do_lo = desc_k_major(sm.dout);
+    auto score = [&](int j) { product_abt<D>(lead, tmem + (j & 1) * kBlock, q_lo, desc_k_major(sm.k[j % 3]), &sm.s_full[j & 1]); };
+    auto dprob = [&](int j) {
+      product_abt<D>(lead, tmem + DP_COL, do_lo, desc_k_major(sm.v[j & 1]), &sm.dp_full);
+      commit(lead, &sm.v_empty[j & 1]);
+    };
+    bool ok = mbar_wait_warp(&sm.q_full, 0, p.status, kTimeoutFull) && mbar_wait_warp(&sm.k_full[0], 0, p.status, kTimeoutFull);
+    if (ok) {
+      tc_fence_after();
+      score(0);
+      ok = mbar_wait_warp(&sm.v_full[0], 0, p.status, kTimeoutFull);
     }
+    if (ok) {
+      tc_fence_after();
+      dprob(0);
+      if (n > 1) {
+        ok = mbar_wait_warp(&sm.k_full[1], 0, p.status, kTimeoutFull);
+        if (ok) {
+          tc_fence_after();
+          score(1);
+        }
+      }
+    }
+    for (int j = 0; ok && j < n; ++j) {
+      if (j + 1 < n) {
+        if (!mbar_wait_warp(&sm.v_full[(j + 1) & 1], ((j + 1) >> 1) & 1, p.status, kTimeoutFull)) break;
+        if (!mbar_wait_warp(&sm.dp_taken, j & 1, p.status, kTimeoutFull)) break;
+        tc_fence_after();
+        dprob(j + 1);
+      }
+      if (!mbar_wait_warp(&sm.ds_ready, j & 1, p.status, kTimeoutFull)) break;
+      tc_fence_after();
+      product_ab<D, kCols>(lead, tmem + DQ_COL, tmem + (j & 1) * kBlock, desc_mn_major(sm.k[j % 3]), j > 0);
+      commit(lead, &sm.k_empty[j % 3]);
+      if (j + 2 < n) {  // in order after dQ(j), which reads dS from the same columns
+        if (!mbar_wait_warp(&sm.k_full[(j + 2) % 3], ((j + 2) / 3) & 1, p.status, kTimeoutFull)) break;
+        tc_fence_after();
+        score(j + 2);
+      }
+    }
+    commit(lead, &sm.done);
+    mbar_wait_warp(&sm.done, 0, p.status, kTimeoutOther);
   } else if (warp >= 4) {
-    // ------------------------------------------------ compute warpgroups: 64 keys each, one query per thread
-    const int half = (warp - 4) >> 2;
+    // ------------------------------------------------ compute warpgroups: 32 keys each, one query per thread
+    const int wg = (warp - 4) >> 2;
     const int quarter = warp & 3;
     const int r = quarter * 32 + lane;
     const uint32_t lane_addr = static_cast<uint32_t>(quarter * 32) << 16;
     const int qi = i0 + r;
-    const int lim = min(qi + s.off, s.klen - 1);  // last key this row sees
+    const int seen = min(qi + s.off, s.klen - 1) + 1 - wg * kCols;  // minus a tile's first key: columns below it are seen
     const long long vo = h * p.pad_rows + s.pad_row0 + qi;
-    const float lse2 = p.lse2[vo], delta = p.delta[vo];
+    const float neg_lse2 = p.neg_lse2[vo], neg_delta = p.neg_delta[vo];
+    const unsigned long long nl2 = f2_pack(neg_lse2, neg_lse2), nd2 = f2_pack(neg_delta, neg_delta);
+    const uint32_t dp_addr = tmem + lane_addr + DP_COL + wg * kCols;
     bool ok = true;
     for (int j = 0; j < n; ++j) {
-      const uint32_t s_addr = tmem + lane_addr + (j & 1) * kBlock + half * kHalf;
-      const uint32_t dp_addr = tmem + lane_addr + DP_COL + half * kHalf;
+      const uint32_t s_addr = tmem + lane_addr + (j & 1) * kBlock + wg * kCols;
       if (!mbar_wait_warp(&sm.s_full[j & 1], (j >> 1) & 1, p.status, kTimeoutAccFull)) {
         ok = false;
         break;
       }
       tc_fence_after();
-      float pv[kHalf];
+      unsigned long long pv[kCols / 2];
       {
-        uint32_t raw[kHalf];
-        tmem_ld32(s_addr, *reinterpret_cast<uint32_t(*)[32]>(&raw[0]));
-        tmem_ld32(s_addr + 32, *reinterpret_cast<uint32_t(*)[32]>(&raw[32]));
+        uint32_t raw[kCols];
+        tmem_ld32(s_addr, raw);
         tmem_ld_wait();
-        probabilities<false>(raw, pv, p.scale_log2, nullptr, lse2);
+        probabilities(raw, pv, p.scale_log2, [&](int) { return nl2; });
       }
       if (!mbar_wait_warp(&sm.dp_full, j & 1, p.status, kTimeoutAccFull)) {
         ok = false;
         break;
       }
       tc_fence_after();
-      uint32_t d0[32], d1[32];
-      tmem_ld32(dp_addr, d0);
-      tmem_ld32(dp_addr + 32, d1);
+      uint32_t d[kCols];
+      tmem_ld32(dp_addr, d);
       tmem_ld_wait();
       tc_fence_before();
       mbar_arrive(&sm.dp_taken);
-      const int hi = lim + 1 - j * kBlock - half * kHalf;  // columns below hi are seen
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        const uint32_t(&cur)[32] = c ? d1 : d0;
-        float ds[32];
+      for (int i = 0; i < kCols / 2; ++i)
+        pv[i] = f2_mul(pv[i], f2_add(f2_pack(__uint_as_float(d[2 * i]), __uint_as_float(d[2 * i + 1])), nd2));
+      if (seen - j * kBlock < kCols) keep_columns(pv, 0, seen - j * kBlock);
+      uint32_t pk[16];
 #pragma unroll
-        for (int i = 0; i < 32; ++i) ds[i] = pv[c * 32 + i] * (__uint_as_float(cur[i]) - delta);
-        if (hi < kHalf) {
-#pragma unroll
-          for (int i = 0; i < 32; ++i) ds[i] = c * 32 + i < hi ? ds[i] : 0.0f;
-        }
-        uint32_t pk[16];
-#pragma unroll
-        for (int i = 0; i < 16; ++i) pk[i] = pack_bf16x2(ds[2 * i], ds[2 * i + 1]);
-        tmem_st16(s_addr + c * 16, pk);
-      }
+      for (int i = 0; i < 16; ++i) pk[i] = pack_pair(pv[i]);
+      tmem_st16(s_addr, pk);
       if ((j + 1) * kBlock > s.klen) {  // the last key tile ends inside: K's rows of the next sequence (S(j) has read them)
-        clear_rows<D>(sm.k[j % 3], s.klen - j * kBlock, threadIdx.x - 128, 256);
+        clear_rows<D>(sm.k[j % 3], s.klen - j * kBlock, threadIdx.x - 128, kComputeThreads);
         fence_proxy_async();
       }
       tmem_st_wait();
@@ -637,9 +598,9 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     }
     if (ok && mbar_wait_warp(&sm.done, 0, p.status, kTimeoutAccFull)) {
       tc_fence_after();
-      constexpr int DH = D / 2;
-      store_row<DH>(tmem + lane_addr + DQ_COL + half * DH, p.d0 + (static_cast<long long>(s.q0) + qi) * p.d0_n + h * p.d0_h + half * DH,
-                    p.scale, qi < s.qlen);
+      constexpr int W = D / kGroups;
+      store_row<W>(tmem + lane_addr + DQ_COL + wg * W, p.d0 + (static_cast<long long>(s.q0) + qi) * p.d0_n + h * p.d0_h + wg * W,
+                   p.scale, qi < s.qlen);
     }
   }
   tc_fence_before();
@@ -707,10 +668,10 @@ void packed_attn_bwd(torch::Tensor q, torch::Tensor k, torch::Tensor v, torch::T
   p.Hq = static_cast<int>(Hq);
   p.Hkv = static_cast<int>(Hkv);
   p.pad_rows = pad_slots(Nq, B) * kBlock;
-  float* lse2 = stats.data_ptr<float>();
-  float* delta = lse2 + Hq * p.pad_rows;
-  p.lse2 = lse2;
-  p.delta = delta;
+  float* neg_lse2 = stats.data_ptr<float>();
+  float* neg_delta = neg_lse2 + Hq * p.pad_rows;
+  p.neg_lse2 = neg_lse2;
+  p.neg_delta = neg_delta;
   p.scale = static_cast<float>(scale);
   p.scale_log2 = static_cast<float>(scale * 1.4426950408889634);
   p.status = status;
@@ -718,9 +679,9 @@ void packed_attn_bwd(torch::Tensor q, torch::Tensor k, torch::Tensor v, torch::T
                     tdo = head_map_3d(dout, kBlock, "dout");
   // dQ's list first: it checks the offsets, and a bad packing leaves every entry empty
   schedule(p.pk, kQueryTiles, list, static_cast<int>(q_entries), status, st);
-  packed_stats_kernel<<<static_cast<unsigned>(pad_slots(Nq, B)), 256, 0, st>>>(
+  packed_stats_kernel<<<static_cast<unsigned>(pad_slots(Nq, B) * (kBlock / kStatsRows)), 256, 0, st>>>(
       p.pk, list, reinterpret_cast<const __nv_bfloat16*>(o.data_ptr()), reinterpret_cast<const __nv_bfloat16*>(dout.data_ptr()),
-      lse.data_ptr<float>(), lse2, delta, p.pad_rows, p.Hq, static_cast<int>(D));
+      lse.data_ptr<float>(), neg_lse2, neg_delta, p.pad_rows, p.Hq, static_cast<int>(D));
   TT_CUDA_CHECK(cudaGetLastError());
   auto launch = [&](auto kern, size_t smem, int64_t blocks) {
     TT_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));

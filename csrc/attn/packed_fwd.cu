@@ -4,10 +4,13 @@
 //   o_i = sum_{j <= i + len_k - len_q} softmax_j(scale q_i . k_j) v_j   within one sequence;
 //   query head h reads kv head h / (Hq / Hkv); queries that see no key get zeros.
 //
-// One CTA per (sequence, pair of 128-query tiles, query head).  Warp 0 loads Q once and streams
-// K/V tiles by TMA, warp 1 issues the MMAs for both query tiles in turn, warps 4-7 and 8-11 are
-// the softmax of one query tile each (one row per thread, scores in TMEM, P written back over
-// them as the A operand of O += P V).  A last, partial key tile takes rows of the next sequence:
+// One CTA per two 128-query tiles that read the same keys: the same tile of two neighbouring query heads of a
+// kv head where a group has an even number of them (both tiles see as many keys, and a sequence of one tile
+// fills both), else two neighbouring tiles of one head.  Warp 0 loads Q once and streams
+// K/V tiles by TMA, warp 1 issues the MMAs for both query tiles in turn, and two warpgroups each
+// (warps 4-11, 12-19) are the softmax of one query tile: a thread has 64 scores of one row in
+// registers, the two threads of a row share their maxima through shared memory, and P goes back
+// over the scores in TMEM as the A operand of O += P V.  A last, partial key tile takes rows of the next sequence:
 // their probabilities are zero, but zero times an infinity or NaN of a neighbour would not be, so
 // the softmax warps clear those rows of V before the product.
 #include "attn/packed.cuh"
@@ -94,13 +97,18 @@ void schedule(const Packing& p, ScheduleKind kind, int2* list, int capacity, int
 }
 
 // ----------------------------------------------------------------- forward
-constexpr int kThreads = 384;
+constexpr int kThreads = 640;
+constexpr int kHalf = kBlock / 2;  // score columns of a softmax warpgroup
+// Registers per thread after setmaxnreg: the launch gives 96 each, the first warpgroup hands 32 to the other four.
+constexpr int kRegIssue = 64, kRegSoftmax = 104;
+static_assert(kRegIssue + 4 * kRegSoftmax <= 5 * 96, "register split exceeds the launch");
 constexpr float kRescale = 8.0f;  // log2 units the running maximum may lag behind
 
 struct FwdParams {
   Packing pk;
   const int2* list;
   int Hq, Hkv;
+  int head_pairs;    // a CTA's two tiles: 1 one tile of two heads, 0 two tiles of one head
   __nv_bfloat16* o;  // [Nq, Hq, D] contiguous
   float* lse;        // [Hq, Nq] natural log (may be null)
   float scale_log2;
@@ -117,6 +125,7 @@ struct FwdSmem {
   uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2];
   uint64_t s_full[2], p_full[2], o_done[2];
   uint64_t done;
+  float row_max[2][2][2][kBlock];  // [tile parity][query tile][column half][row]; the row sums at the end
   uint32_t tmem_slot;
 };
 
@@ -126,23 +135,25 @@ __global__ void __launch_bounds__(kThreads, 1)
                       const __grid_constant__ CUtensorMap tmV, const FwdParams p) {
   static_assert(D == 64 || D == 128, "head_dim must be 64 or 128");
   constexpr uint32_t TILE = FwdSmem<D>::TILE;
-  constexpr uint32_t IDESC_QK = idesc_bf16_f32(kBlock, kBlock, false, false);
-  constexpr uint32_t IDESC_PV = idesc_bf16_f32(kBlock, D, false, true);
   constexpr uint32_t TMEM_COLS = 512;
-  // TMEM: S/P of tile x at columns [128 x, +128) (P: bf16 pairs in the first 64), O of tile x at 256 + x D.
+  // TMEM: S/P of tile x at columns [128 x, +128) (P: bf16 pairs, each half over the first 32 columns of its scores),
+  // O of tile x at 256 + x D.
   auto S_COL = [](int x) { return static_cast<uint32_t>(x * kBlock); };
   auto O_COL = [](int x) { return static_cast<uint32_t>(2 * kBlock + x * D); };
 
-  const int2 entry = p.list[blockIdx.x / p.Hq];
+  const int units = p.head_pairs ? p.Hq / 2 : p.Hq;
+  const int2 entry = p.list[blockIdx.x / units];
   if (entry.x < 0) return;  // past the end of the list (uniform over the block, nothing allocated)
-  const int h = static_cast<int>(blockIdx.x) % p.Hq;
-  const int g = h / (p.Hq / p.Hkv);
+  const int h0 = static_cast<int>(blockIdx.x) % units * (p.head_pairs ? 2 : 1);
+  const int g = h0 / (p.Hq / p.Hkv);
   const Seq s = sequence(p.pk, entry.x);
   const bool extra = entry.x == p.pk.B;
-  const int i0 = entry.y * 2 * kBlock;  // first query of the pair
+  // tile x: head h0 + x dh, queries from i0 + x di
+  const int dh = p.head_pairs ? 1 : 0, di = p.head_pairs ? 0 : kBlock;
+  const int i0 = entry.y * (p.head_pairs ? kBlock : 2 * kBlock);
   int n_x[2];
   n_x[0] = key_tiles(s, extra, i0, kBlock);
-  n_x[1] = key_tiles(s, extra, i0 + kBlock, kBlock);
+  n_x[1] = key_tiles(s, extra, i0 + di, kBlock);
   const int n_max = max(n_x[0], n_x[1]);
 
   extern __shared__ uint8_t smem_raw[];
@@ -150,15 +161,17 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   if (n_max == 0) {  // no key is seen: zeros
-    const int rows = min(2 * kBlock, s.qlen - i0);
     constexpr int NU = D / 8;
-    for (int i = threadIdx.x; i < rows * NU; i += kThreads) {
-      const long long row = s.q0 + i0 + i / NU;
-      reinterpret_cast<uint4*>(p.o + (row * p.Hq + h) * D)[i % NU] = make_uint4(0u, 0u, 0u, 0u);
+    for (int x = 0; x < 2; ++x) {
+      const int first = i0 + x * di, rows = min(kBlock, s.qlen - first);
+      for (int i = threadIdx.x; i < rows * NU; i += kThreads) {
+        const long long row = s.q0 + first + i / NU;
+        reinterpret_cast<uint4*>(p.o + (row * p.Hq + h0 + x * dh) * D)[i % NU] = make_uint4(0u, 0u, 0u, 0u);
+      }
+      if (p.lse != nullptr)
+        for (int i = threadIdx.x; i < rows; i += kThreads)
+          p.lse[static_cast<long long>(h0 + x * dh) * p.pk.Nq + s.q0 + first + i] = -INFINITY;
     }
-    if (p.lse != nullptr)
-      for (int i = threadIdx.x; i < rows; i += kThreads)
-        p.lse[static_cast<long long>(h) * p.pk.Nq + s.q0 + i0 + i] = -INFINITY;
     return;
   }
   // rows past the sequence in its last key tile, where it is one of those seen
@@ -177,7 +190,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&sm.v_full[i], 1);
       mbar_init(&sm.v_empty[i], 1);
       mbar_init(&sm.s_full[i], 1);
-      mbar_init(&sm.p_full[i], 128);
+      mbar_init(&sm.p_full[i], 256);
       mbar_init(&sm.o_done[i], 1);
     }
     mbar_init(&sm.done, 1);
@@ -192,6 +205,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   tc_fence_after();
   const uint32_t tmem = sm.tmem_slot;
 
+  if (warp < 4) {
+  setmaxnreg_dec<kRegIssue>();
   if (warp == 0) {
     if (lane == 0) {
       // ------------------------------------------------ TMA producer
@@ -200,7 +215,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int x = 0; x < 2; ++x)
 #pragma unroll
         for (int c = 0; c < D / 64; ++c)
-          tma_load_3d(sm.q[x] + c * kBlock * 128, &tmQ, &sm.q_full, c * 64, h, s.q0 + i0 + x * kBlock);
+          tma_load_3d(sm.q[x] + c * kBlock * 128, &tmQ, &sm.q_full, c * 64, h0 + x * dh, s.q0 + i0 + x * di);
       for (int j = 0; j < n_max; ++j) {
         const int st = j & 1;
         const uint32_t ph = (j >> 1) & 1;
@@ -222,175 +237,130 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     }
   } else if (warp == 1) {
-    if (lane == 0) {
-      // ------------------------------------------------ MMA issuer, the two query tiles in turn
-      auto qk = [&](int x, int j) {
-        const uint32_t q_base = smem_u32(sm.q[x]);
-        const uint32_t k_base = smem_u32(sm.k[j & 1]);
-#pragma unroll
-        for (int kk = 0; kk < D / 16; ++kk) {
-          const uint32_t off = (kk >> 2) * (kBlock * 128) + (kk & 3) * 32;
-          umma_f16_ss(tmem + S_COL(x), sdesc_sw128(q_base + off, 16, 1024), sdesc_sw128(k_base + off, 16, 1024),
-                      IDESC_QK, kk > 0 ? 1u : 0u);
-        }
-        umma_commit(&sm.s_full[x]);
-      };
-      auto pv = [&](int x, int j) {
-        const uint32_t v_base = smem_u32(sm.v[j & 1]);
-#pragma unroll
-        for (int kk = 0; kk < kBlock / 16; ++kk)
-          umma_f16_ts(tmem + O_COL(x), tmem + S_COL(x) + kk * 8, sdesc_sw128(v_base + kk * 2048, kBlock * 128, 1024),
-                      IDESC_PV, (j > 0 || kk > 0) ? 1u : 0u);
-        umma_commit(&sm.o_done[x]);
-      };
-      bool ok = mbar_wait(&sm.q_full, 0, p.status, kTimeoutFull) && mbar_wait(&sm.k_full[0], 0, p.status, kTimeoutFull);
-      if (ok) {
-        tc_fence_after();
-        for (int x = 0; x < 2; ++x)
-          if (n_x[x] > 0) qk(x, 0);
-        umma_commit(&sm.k_empty[0]);
-      }
-      for (int j = 0; ok && j < n_max; ++j) {
-        const bool next = j + 1 < n_max;
-        if (!mbar_wait(&sm.v_full[j & 1], (j >> 1) & 1, p.status, kTimeoutFull)) break;
-        if (next && !mbar_wait(&sm.k_full[(j + 1) & 1], ((j + 1) >> 1) & 1, p.status, kTimeoutFull)) break;
-        tc_fence_after();
-        for (int x = 0; x < 2; ++x) {
-          if (j < n_x[x]) {
-            if (!mbar_wait(&sm.p_full[x], j & 1, p.status, kTimeoutFull)) {
-              ok = false;
-              break;
-            }
-            tc_fence_after();
-            pv(x, j);
-          }
-          if (j + 1 < n_x[x]) qk(x, j + 1);  // in order after PV(x, j), which read P from these columns
-        }
-        if (!ok) break;
-        umma_commit(&sm.v_empty[j & 1]);
-        if (next) umma_commit(&sm.k_empty[(j + 1) & 1]);
-      }
-      umma_commit(&sm.done);
-      mbar_wait(&sm.done, 0, p.status, kTimeoutOther);
+    // ------------------------------------------------ MMA issuer, the two query tiles in turn
+    const bool lead = elect_one();
+    auto qk = [&](int x, int j) {
+      product_abt<D>(lead, tmem + S_COL(x), desc_k_major(sm.q[x]), desc_k_major(sm.k[j & 1]), &sm.s_full[x]);
+    };
+    auto pv = [&](int x, int j) {
+      product_ab<D, kHalf>(lead, tmem + O_COL(x), tmem + S_COL(x), desc_mn_major(sm.v[j & 1]), j > 0);
+      commit(lead, &sm.o_done[x]);
+    };
+    bool ok = mbar_wait_warp(&sm.q_full, 0, p.status, kTimeoutFull) && mbar_wait_warp(&sm.k_full[0], 0, p.status, kTimeoutFull);
+    if (ok) {
+      tc_fence_after();
+      for (int x = 0; x < 2; ++x)
+        if (n_x[x] > 0) qk(x, 0);
+      commit(lead, &sm.k_empty[0]);
     }
-  } else if (warp >= 4) {
-    // ------------------------------------------------ softmax warpgroups: x = 0 (warps 4-7), 1 (warps 8-11)
-    const int x = (warp - 4) >> 2;
+    for (int j = 0; ok && j < n_max; ++j) {
+      const bool next = j + 1 < n_max;
+      if (!mbar_wait_warp(&sm.v_full[j & 1], (j >> 1) & 1, p.status, kTimeoutFull)) break;
+      if (next && !mbar_wait_warp(&sm.k_full[(j + 1) & 1], ((j + 1) >> 1) & 1, p.status, kTimeoutFull)) break;
+      tc_fence_after();
+      for (int x = 0; x < 2; ++x) {
+        if (j < n_x[x]) {
+          if (!mbar_wait_warp(&sm.p_full[x], j & 1, p.status, kTimeoutFull)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          pv(x, j);
+        }
+        if (j + 1 < n_x[x]) qk(x, j + 1);  // in order after PV(x, j), which read P from these columns
+      }
+      if (!ok) break;
+      commit(lead, &sm.v_empty[j & 1]);
+      if (next) commit(lead, &sm.k_empty[(j + 1) & 1]);
+    }
+    commit(lead, &sm.done);
+    mbar_wait_warp(&sm.done, 0, p.status, kTimeoutOther);
+  }
+  } else {
+    setmaxnreg_inc<kRegSoftmax>();
+    // ------------------------------------------------ softmax: query tile x, column half `half`, one row per thread
+    const int x = (warp - 4) >> 3;
+    const int half = ((warp - 4) >> 2) & 1;
     const int quarter = warp & 3;
     const int r = quarter * 32 + lane;
-    const int qi = i0 + x * kBlock + r;  // query within the sequence
+    const int qi = i0 + x * di + r;  // query within the sequence
+    const int h = h0 + x * dh;
     const uint32_t lane_addr = static_cast<uint32_t>(quarter * 32) << 16;
-    const uint32_t s_addr = tmem + lane_addr + S_COL(x);
-    const uint32_t o_addr = tmem + lane_addr + O_COL(x);
+    const uint32_t s_addr = tmem + lane_addr + S_COL(x) + half * kHalf;
+    const uint32_t o_addr = tmem + lane_addr + O_COL(x) + half * (D / 2);
     const int lim = min(qi + s.off, s.klen - 1);  // last key this row sees (negative: none)
     const int n = n_x[x];
     const float sl2 = p.scale_log2;
-    float m_ref = -INFINITY;  // reference maximum, scaled log2 units
-    float l = 0.0f;
+    float m_ref = -INFINITY;  // reference maximum, scaled log2 units (the same in both threads of a row)
+    float l = 0.0f;           // sum over this thread's columns
+    // Both warpgroups of a query tile meet once per key tile: after a wait that gave up they go on meeting (and
+    // compute nothing), so that neither is left waiting for the other.
+    auto meet = [&]() {
+      if (x == 0) asm volatile("bar.sync 1, 256;" ::: "memory");
+      else asm volatile("bar.sync 2, 256;" ::: "memory");
+    };
     bool ok = true;
     for (int j = 0; j < n; ++j) {
-      if (!mbar_wait_warp(&sm.s_full[x], j & 1, p.status, kTimeoutAccFull)) {
-        ok = false;
-        break;
+      if (ok) ok = mbar_wait_warp(&sm.s_full[x], j & 1, p.status, kTimeoutAccFull);
+      if (!ok) {
+        meet();
+        continue;
       }
       tc_fence_after();
-      const int key0 = j * kBlock;
-      const bool need_mask = key0 + kBlock - 1 > lim;
-      // Scores in four chunks of 32 columns, each chunk's TMEM load under the previous one's math.
-      // The reference maximum rises only when a chunk's maximum exceeds it by more than 2^8, so no
-      // exponential overflows; what was computed under an older reference is rescaled after.
-      const float m_start = m_ref;
-      float cref[4], csum[4];
-      {
-        uint32_t bufA[32], bufB[32];
-        tmem_ld32(s_addr, bufA);
-        tmem_ld_wait();
+      uint32_t raw[kHalf];
+      tmem_ld32(s_addr, *reinterpret_cast<uint32_t(*)[32]>(&raw[0]));
+      tmem_ld32(s_addr + 32, *reinterpret_cast<uint32_t(*)[32]>(&raw[32]));
+      tmem_ld_wait();
+      const int left = lim - j * kBlock - half * kHalf;  // columns up to `left` are seen
+      if (left < kHalf - 1) {
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          uint32_t(&cur)[32] = (c & 1) ? bufB : bufA;
-          uint32_t(&nxt)[32] = (c & 1) ? bufA : bufB;
-          if (c < 3) tmem_ld32(s_addr + (c + 1) * 32, nxt);
-          float v[32];
+        for (int i = 0; i < kHalf; ++i) raw[i] = i > left ? 0xff800000u : raw[i];  // -inf
+      }
+      float mq[4];
 #pragma unroll
-          for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(cur[i]);
-          if (need_mask) {
+      for (int q = 0; q < 4; ++q) {
+        mq[q] = fmax3(__uint_as_float(raw[q]), __uint_as_float(raw[q + 4]), __uint_as_float(raw[q + 8]));
 #pragma unroll
-            for (int i = 0; i < 32; ++i) v[i] = key0 + c * 32 + i > lim ? -INFINITY : v[i];
+        for (int i = q + 12; i + 4 < kHalf; i += 8) mq[q] = fmax3(mq[q], __uint_as_float(raw[i]), __uint_as_float(raw[i + 4]));
+        mq[q] = fmaxf(mq[q], __uint_as_float(raw[q + kHalf - 4]));
+      }
+      const float own = fmax3(mq[0], mq[1], fmaxf(mq[2], mq[3]));
+      sm.row_max[j & 1][x][half][r] = own;
+      meet();
+      const float m_tile = fmaxf(own, sm.row_max[j & 1][x][half ^ 1][r]) * sl2;
+      // The reference rises only when the tile's maximum exceeds it by more than 2^8: no exponential overflows,
+      // and after the first tiles of a row almost none has to be rescaled.
+      const float m_old = m_ref;
+      if (m_tile > m_ref + kRescale) m_ref = m_tile;  // also the first visible tile (m_ref = -inf)
+      const float neg_m = (m_ref == -INFINITY) ? 0.0f : -m_ref;
+      const unsigned long long s2 = f2_pack(sl2, sl2), nm2 = f2_pack(neg_m, neg_m);
+      unsigned long long sa = 0ull, sb = 0ull;  // pairs of partial sums
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        uint32_t pk[16];
+#pragma unroll
+        for (int i = 0; i < 32; i += 2) {
+          float e0, e1;
+          f2_unpack(f2_fma(f2_pack(__uint_as_float(raw[c * 32 + i]), __uint_as_float(raw[c * 32 + i + 1])), s2, nm2), e0, e1);
+          if ((i & 7) == 6) {  // one pair of four on the FMA pipe, so that MUFU does not bound the tile
+            exp2_poly2(e0, e1);
+          } else {
+            e0 = ex2_mufu(e0);
+            e1 = ex2_mufu(e1);
           }
-          float e[32];
-          float mq[4];
-#pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            float m = fmax3(v[q], v[q + 4], v[q + 8]);
-            m = fmax3(m, v[q + 12], v[q + 16]);
-            m = fmax3(m, v[q + 20], v[q + 24]);
-            mq[q] = fmaxf(m, v[q + 28]);
-          }
-          const float mcs = fmax3(mq[0], mq[1], fmaxf(mq[2], mq[3])) * sl2;
-          if (mcs > m_ref + kRescale) m_ref = mcs;  // also the first visible chunk (m_ref = -inf)
-          const float neg_m = (m_ref == -INFINITY) ? 0.0f : -m_ref;
-          const unsigned long long s2 = f2_pack(sl2, sl2), nm2 = f2_pack(neg_m, neg_m);
-#pragma unroll
-          for (int i = 0; i < 32; i += 2) {
-            const unsigned long long r2 = f2_fma(f2_pack(v[i], v[i + 1]), s2, nm2);
-            f2_unpack(r2, e[i], e[i + 1]);
-          }
-          // two of eight exponentials on the FMA pipe, so that MUFU does not bound the tile
-#pragma unroll
-          for (int i = 0; i < 32; i += 2) {
-            if ((i & 7) == 6) {
-              exp2_poly2(e[i], e[i + 1]);
-            } else {
-              e[i] = ex2_mufu(e[i]);
-              e[i + 1] = ex2_mufu(e[i + 1]);
-            }
-          }
-          unsigned long long sa = f2_pack(e[0], e[1]), sb = f2_pack(e[2], e[3]);
-#pragma unroll
-          for (int i = 4; i < 32; i += 4) {
-            sa = f2_add(sa, f2_pack(e[i], e[i + 1]));
-            sb = f2_add(sb, f2_pack(e[i + 2], e[i + 3]));
-          }
-          float a0, a1;
-          f2_unpack(f2_add(sa, sb), a0, a1);
-          csum[c] = a0 + a1;
-          cref[c] = m_ref;
-          uint32_t pk[16];
-#pragma unroll
-          for (int i = 0; i < 16; ++i) pk[i] = pack_bf16x2(e[2 * i], e[2 * i + 1]);
-          tmem_st16(s_addr + c * 16, pk);
-          if (c < 3) tmem_ld_wait();
+          if (i & 2) sb = f2_add(sb, f2_pack(e0, e1));
+          else sa = f2_add(sa, f2_pack(e0, e1));
+          pk[i >> 1] = pack_bf16x2(e0, e1);
         }
+        tmem_st16(s_addr + c * 16, pk);
       }
-      float rs = 0.0f;
-      float cf[4];
-      bool fix = false;
+      float s0, s1;
+      f2_unpack(f2_add(sa, sb), s0, s1);
+      const float alpha = (m_old == m_ref) ? 1.0f : ex2_mufu(m_old - m_ref);
+      l = l * alpha + (s0 + s1);
+      if (__any_sync(0xffffffffu, j > 0 && alpha != 1.0f)) {  // rare: O under an older reference, this half of its columns
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        cf[c] = (cref[c] == m_ref) ? 1.0f : ex2_mufu(cref[c] - m_ref);
-        fix |= cf[c] != 1.0f;
-        rs = fmaf(csum[c], cf[c], rs);
-      }
-      if (__any_sync(0xffffffffu, fix)) {  // rare: P chunks under an older reference
-        tmem_st_wait();
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          uint32_t pv[16];
-          tmem_ld16(s_addr + c * 16, pv);
-          tmem_ld_wait();
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const float2 f = unpack_bf16x2(pv[i]);
-            pv[i] = pack_bf16x2(f.x * cf[c], f.y * cf[c]);
-          }
-          tmem_st16(s_addr + c * 16, pv);
-        }
-      }
-      const float alpha = (m_start == m_ref) ? 1.0f : ex2_mufu(m_start - m_ref);
-      l = l * alpha + rs;
-      if (__any_sync(0xffffffffu, j > 0 && alpha != 1.0f)) {  // rare: O under an older reference
-#pragma unroll
-        for (int c = 0; c < D; c += 16) {
+        for (int c = 0; c < D / 2; c += 16) {
           uint32_t ov[16];
           tmem_ld16(o_addr + c, ov);
           tmem_ld_wait();
@@ -403,9 +373,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (clean && x == cleaner && j == n_max - 1) {
         if (!mbar_wait_warp(&sm.v_full[j & 1], (j >> 1) & 1, p.status, kTimeoutFull)) {
           ok = false;
-          break;
+          continue;
         }
-        clear_rows<D>(sm.v[j & 1], s.klen - key0, r, kBlock);
+        clear_rows<D>(sm.v[j & 1], s.klen - j * kBlock, half * kBlock + r, 2 * kBlock);
         fence_proxy_async();
       }
       tmem_st_wait();
@@ -415,35 +385,40 @@ __global__ void __launch_bounds__(kThreads, 1)
     // ------------------------------------------------ O / l and the log-sum-exp
     const bool row_ok = qi < s.qlen;
     const long long row = s.q0 + qi;
-    __nv_bfloat16* orow = p.o + (row * p.Hq + h) * D;
+    __nv_bfloat16* orow = p.o + (row * p.Hq + h) * D + half * (D / 2);
     if (n == 0) {
       if (row_ok) {
 #pragma unroll
-        for (int c = 0; c < D / 8; ++c) reinterpret_cast<uint4*>(orow)[c] = make_uint4(0u, 0u, 0u, 0u);
-        if (p.lse != nullptr) p.lse[static_cast<long long>(h) * p.pk.Nq + row] = -INFINITY;
+        for (int c = 0; c < D / 16; ++c) reinterpret_cast<uint4*>(orow)[c] = make_uint4(0u, 0u, 0u, 0u);
+        if (p.lse != nullptr && half == 0) p.lse[static_cast<long long>(h) * p.pk.Nq + row] = -INFINITY;
       }
-    } else if (ok && mbar_wait_warp(&sm.o_done[x], (n - 1) & 1, p.status, kTimeoutAccFull)) {
-      tc_fence_after();
-      const bool seen = lim >= 0;
-      const float inv_l = 1.0f / l;
+    } else {
+      if (ok) ok = mbar_wait_warp(&sm.o_done[x], (n - 1) & 1, p.status, kTimeoutAccFull);
+      // the last tile's maxima are in [(n - 1) & 1]: the sums go into the other buffer
+      sm.row_max[n & 1][x][half][r] = l;
+      meet();
+      if (ok) {
+        l += sm.row_max[n & 1][x][half ^ 1][r];
+        tc_fence_after();
+        const bool seen = lim >= 0;
+        const float inv_l = 1.0f / l;
 #pragma unroll
-      for (int c = 0; c < D; c += 32) {
-        uint32_t ov[32];
-        tmem_ld32(o_addr + c, ov);
-        tmem_ld_wait();
-        if (row_ok) {
-          uint4* dst = reinterpret_cast<uint4*>(orow + c);
-          float f[32];
+        for (int c = 0; c < D / 2; c += 32) {
+          uint32_t ov[32];
+          tmem_ld32(o_addr + c, ov);
+          tmem_ld_wait();
+          if (row_ok) {
+            uint32_t w[16];
 #pragma unroll
-          for (int i = 0; i < 32; ++i) f[i] = seen ? __uint_as_float(ov[i]) * inv_l : 0.0f;
+            for (int i = 0; i < 16; ++i)
+              w[i] = seen ? pack_bf16x2(__uint_as_float(ov[2 * i]) * inv_l, __uint_as_float(ov[2 * i + 1]) * inv_l) : 0u;
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
-            dst[i] = make_uint4(pack_bf16x2(f[8 * i], f[8 * i + 1]), pack_bf16x2(f[8 * i + 2], f[8 * i + 3]),
-                                pack_bf16x2(f[8 * i + 4], f[8 * i + 5]), pack_bf16x2(f[8 * i + 6], f[8 * i + 7]));
+            for (int i = 0; i < 4; ++i) reinterpret_cast<uint4*>(orow + c)[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+          }
         }
+        if (row_ok && half == 0 && p.lse != nullptr)
+          p.lse[static_cast<long long>(h) * p.pk.Nq + row] = seen ? (m_ref + log2f(l)) * 0.69314718055994531f : -INFINITY;
       }
-      if (row_ok && p.lse != nullptr)
-        p.lse[static_cast<long long>(h) * p.pk.Nq + row] = seen ? (m_ref + log2f(l)) * 0.69314718055994531f : -INFINITY;
     }
   }
 
@@ -504,12 +479,14 @@ void packed_attn_fwd(torch::Tensor q, torch::Tensor k, torch::Tensor v, torch::T
   p.scale_log2 = static_cast<float>(scale * 1.4426950408889634);
   p.status = device_status_ptr(q.get_device());
   const CUtensorMap tq = head_map_3d(q, kBlock, "q"), tk = head_map_3d(k, kBlock, "k"), tv = head_map_3d(v, kBlock, "v");
-  const int64_t entries = max_tiles(Nq, B, 2 * kBlock);
-  TT_CHECK(entries * Hq < (1LL << 31), "packed_attn: too many tiles");
-  schedule(p.pk, kQueryPairs, reinterpret_cast<int2*>(sched.data_ptr<int>()), static_cast<int>(entries), p.status, cur_stream());
+  p.head_pairs = (Hq / Hkv) % 2 == 0 ? 1 : 0;
+  const int64_t entries = max_tiles(Nq, B, p.head_pairs ? kBlock : 2 * kBlock);
+  const int64_t blocks = entries * (p.head_pairs ? Hq / 2 : Hq);
+  TT_CHECK(blocks < (1LL << 31), "packed_attn: too many tiles");
+  schedule(p.pk, p.head_pairs ? kQueryTiles : kQueryPairs, reinterpret_cast<int2*>(sched.data_ptr<int>()), static_cast<int>(entries), p.status, cur_stream());
   auto launch = [&](auto kern, size_t smem) {
     TT_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
-    kern<<<static_cast<unsigned>(entries * Hq), kThreads, smem, cur_stream()>>>(tq, tk, tv, p);
+    kern<<<static_cast<unsigned>(blocks), kThreads, smem, cur_stream()>>>(tq, tk, tv, p);
   };
   if (D == 128) launch(packed_fwd_kernel<128>, sizeof(FwdSmem<128>) + 1024);
   else launch(packed_fwd_kernel<64>, sizeof(FwdSmem<64>) + 1024);
