@@ -42,8 +42,9 @@ __device__ __forceinline__ unsigned long long f2_mul(unsigned long long a, unsig
   return d;
 }
 
-// Probabilities of 32 scores in pairs: 2^(s scale_log2 + add), add = -lse2 of the column (or row).
-template <typename Add>
+// Probabilities of 32 scores in pairs: 2^(s scale_log2 + add), add = -lse2 of the column (or row); kPoly of eight
+// exponentials on the FMA pipe instead of MUFU.
+template <int kPoly, typename Add>
 __device__ __forceinline__ void probabilities(const uint32_t (&raw)[kCols], unsigned long long (&pv)[kCols / 2],
                                               float scale_log2, Add add) {
   const unsigned long long s2 = f2_pack(scale_log2, scale_log2);
@@ -51,7 +52,13 @@ __device__ __forceinline__ void probabilities(const uint32_t (&raw)[kCols], unsi
   for (int i = 0; i < kCols / 2; ++i) {
     float a, b;
     f2_unpack(f2_fma(f2_pack(__uint_as_float(raw[2 * i]), __uint_as_float(raw[2 * i + 1])), s2, add(i)), a, b);
-    pv[i] = f2_pack(ex2_mufu(a), ex2_mufu(b));
+    if ((i & 3) == 3) {
+      exp2_poly2(a, b);
+    } else {
+      a = ex2_mufu(a);
+      b = (kPoly == 3 && (i & 3) == 1) ? exp2_poly(b) : ex2_mufu(b);
+    }
+    pv[i] = f2_pack(a, b);
   }
 }
 __device__ __forceinline__ uint32_t pack_pair(unsigned long long v) {
@@ -327,7 +334,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       tmem_ld32(s_addr, raw);
       const ulonglong2* nl = reinterpret_cast<const ulonglong2*>(sm.neg_lse2[buf] + wg * kCols);
       tmem_ld_wait();
-      probabilities(raw, pv, p.scale_log2, [&](int i) { return (i & 1) ? nl[i >> 1].y : nl[i >> 1].x; });
+      probabilities<3>(raw, pv, p.scale_log2, [&](int i) { return (i & 1) ? nl[i >> 1].y : nl[i >> 1].x; });
       const int lo = key_row - qt * kBlock, hi = end_row - qt * kBlock;
       if (lo > 0 || hi < kCols) keep_columns(pv, lo, hi);
       uint32_t pk[16];
@@ -568,7 +575,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         uint32_t raw[kCols];
         tmem_ld32(s_addr, raw);
         tmem_ld_wait();
-        probabilities(raw, pv, p.scale_log2, [&](int) { return nl2; });
+        probabilities<2>(raw, pv, p.scale_log2, [&](int) { return nl2; });
       }
       if (!mbar_wait_warp(&sm.dp_full, j & 1, p.status, kTimeoutAccFull)) {
         ok = false;

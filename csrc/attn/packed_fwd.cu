@@ -7,10 +7,12 @@
 // One CTA per two 128-query tiles that read the same keys: the same tile of two neighbouring query heads of a
 // kv head where a group has an even number of them (both tiles see as many keys, and a sequence of one tile
 // fills both), else two neighbouring tiles of one head.  Warp 0 loads Q once and streams
-// K/V tiles by TMA, warp 1 issues the MMAs for both query tiles in turn, and two warpgroups each
-// (warps 4-11, 12-19) are the softmax of one query tile: a thread has 64 scores of one row in
-// registers, the two threads of a row share their maxima through shared memory, and P goes back
-// over the scores in TMEM as the A operand of O += P V.  A last, partial key tile takes rows of the next sequence:
+// K/V tiles by TMA, warp 1 issues the MMAs for both query tiles in turn, and four warpgroups (warps
+// 4-19) are the softmax of whichever tile has its scores: a thread takes 32 scores of one row, the
+// four threads of a row share their maxima through shared memory, and P goes back over the scores in
+// TMEM as the A operand of O += P V.  While the softmax works on one tile the tensor core runs the
+// other's products; all four warpgroups on one tile at a time, rather than two on each, because a
+// tile's softmax is on the critical path between its products.  A last, partial key tile takes rows of the next sequence:
 // their probabilities are zero, but zero times an infinity or NaN of a neighbour would not be, so
 // the softmax warps clear those rows of V before the product.
 #include "attn/packed.cuh"
@@ -98,7 +100,10 @@ void schedule(const Packing& p, ScheduleKind kind, int2* list, int capacity, int
 
 // ----------------------------------------------------------------- forward
 constexpr int kThreads = 640;
-constexpr int kHalf = kBlock / 2;  // score columns of a softmax warpgroup
+constexpr int kCols = kBlock / 4;  // score columns of a softmax warpgroup
+constexpr int kSoftmaxThreads = 512;
+constexpr int kPolyEighths = 3;    // exponentials of eight computed on the FMA pipe (2: 167.2 us, 3: 166.0, 4: 166.6, 0: 178.9
+                                   // on 16K packed prompt tokens, 16/4 heads of 128)
 // Registers per thread after setmaxnreg: the launch gives 96 each, the first warpgroup hands 32 to the other four.
 constexpr int kRegIssue = 64, kRegSoftmax = 104;
 static_assert(kRegIssue + 4 * kRegSoftmax <= 5 * 96, "register split exceeds the launch");
@@ -125,7 +130,7 @@ struct FwdSmem {
   uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2];
   uint64_t s_full[2], p_full[2], o_done[2];
   uint64_t done;
-  float row_max[2][2][2][kBlock];  // [tile parity][query tile][column half][row]; the row sums at the end
+  float row_max[2][4][kBlock];  // [query tile][warpgroup][row]; the row sums at the end
   uint32_t tmem_slot;
 };
 
@@ -136,7 +141,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   static_assert(D == 64 || D == 128, "head_dim must be 64 or 128");
   constexpr uint32_t TILE = FwdSmem<D>::TILE;
   constexpr uint32_t TMEM_COLS = 512;
-  // TMEM: S/P of tile x at columns [128 x, +128) (P: bf16 pairs, each half over the first 32 columns of its scores),
+  // TMEM: S/P of tile x at columns [128 x, +128) (P: bf16 pairs, each warpgroup's over the first 16 columns of its scores),
   // O of tile x at 256 + x D.
   auto S_COL = [](int x) { return static_cast<uint32_t>(x * kBlock); };
   auto O_COL = [](int x) { return static_cast<uint32_t>(2 * kBlock + x * D); };
@@ -190,7 +195,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&sm.v_full[i], 1);
       mbar_init(&sm.v_empty[i], 1);
       mbar_init(&sm.s_full[i], 1);
-      mbar_init(&sm.p_full[i], 256);
+      mbar_init(&sm.p_full[i], kSoftmaxThreads);
       mbar_init(&sm.o_done[i], 1);
     }
     mbar_init(&sm.done, 1);
@@ -243,7 +248,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       product_abt<D>(lead, tmem + S_COL(x), desc_k_major(sm.q[x]), desc_k_major(sm.k[j & 1]), &sm.s_full[x]);
     };
     auto pv = [&](int x, int j) {
-      product_ab<D, kHalf>(lead, tmem + O_COL(x), tmem + S_COL(x), desc_mn_major(sm.v[j & 1]), j > 0);
+      product_ab<D, kCols>(lead, tmem + O_COL(x), tmem + S_COL(x), desc_mn_major(sm.v[j & 1]), j > 0);
       commit(lead, &sm.o_done[x]);
     };
     bool ok = mbar_wait_warp(&sm.q_full, 0, p.status, kTimeoutFull) && mbar_wait_warp(&sm.k_full[0], 0, p.status, kTimeoutFull);
@@ -278,146 +283,142 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
   } else {
     setmaxnreg_inc<kRegSoftmax>();
-    // ------------------------------------------------ softmax: query tile x, column half `half`, one row per thread
-    const int x = (warp - 4) >> 3;
-    const int half = ((warp - 4) >> 2) & 1;
+    // ------------------------------------------------ softmax: columns [32 wg, +32) of both tiles, one row of each per thread
+    const int wg = (warp - 4) >> 2;
     const int quarter = warp & 3;
     const int r = quarter * 32 + lane;
-    const int qi = i0 + x * di + r;  // query within the sequence
-    const int h = h0 + x * dh;
     const uint32_t lane_addr = static_cast<uint32_t>(quarter * 32) << 16;
-    const uint32_t s_addr = tmem + lane_addr + S_COL(x) + half * kHalf;
-    const uint32_t o_addr = tmem + lane_addr + O_COL(x) + half * (D / 2);
-    const int lim = min(qi + s.off, s.klen - 1);  // last key this row sees (negative: none)
-    const int n = n_x[x];
     const float sl2 = p.scale_log2;
-    float m_ref = -INFINITY;  // reference maximum, scaled log2 units (the same in both threads of a row)
-    float l = 0.0f;           // sum over this thread's columns
-    // Both warpgroups of a query tile meet once per key tile: after a wait that gave up they go on meeting (and
-    // compute nothing), so that neither is left waiting for the other.
-    auto meet = [&]() {
-      if (x == 0) asm volatile("bar.sync 1, 256;" ::: "memory");
-      else asm volatile("bar.sync 2, 256;" ::: "memory");
-    };
+    constexpr int W = D / 4;                         // columns of O that this thread rescales and writes
+    float m_ref[2] = {-INFINITY, -INFINITY};         // reference maximum, scaled log2 units (the same in a row's four threads)
+    float l[2] = {0.0f, 0.0f};                       // sums over this thread's columns
+    // The warpgroups meet once per tile: after a wait that gave up they go on meeting (and compute nothing), so that
+    // none is left waiting for another.
+    auto meet = [&]() { asm volatile("bar.sync 1, 512;" ::: "memory"); };
     bool ok = true;
-    for (int j = 0; j < n; ++j) {
-      if (ok) ok = mbar_wait_warp(&sm.s_full[x], j & 1, p.status, kTimeoutAccFull);
-      if (!ok) {
+    for (int j = 0; j < n_max; ++j) {
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        if (j >= n_x[x]) continue;
+        if (ok) ok = mbar_wait_warp(&sm.s_full[x], j & 1, p.status, kTimeoutAccFull);
+        if (!ok) {
+          meet();
+          continue;
+        }
+        tc_fence_after();
+        const uint32_t s_addr = tmem + lane_addr + S_COL(x) + wg * kCols;
+        uint32_t raw[kCols];
+        tmem_ld32(s_addr, raw);
+        tmem_ld_wait();
+        const int lim = min(i0 + x * di + r + s.off, s.klen - 1);  // last key this row sees (negative: none)
+        const int left = lim - j * kBlock - wg * kCols;            // columns up to `left` are seen
+        if (left < kCols - 1) {
+#pragma unroll
+          for (int i = 0; i < kCols; ++i) raw[i] = i > left ? 0xff800000u : raw[i];  // -inf
+        }
+        float mq[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          mq[q] = fmax3(__uint_as_float(raw[8 * q]), __uint_as_float(raw[8 * q + 1]), __uint_as_float(raw[8 * q + 2]));
+          mq[q] = fmax3(mq[q], __uint_as_float(raw[8 * q + 3]), __uint_as_float(raw[8 * q + 4]));
+          mq[q] = fmax3(mq[q], __uint_as_float(raw[8 * q + 5]), fmaxf(__uint_as_float(raw[8 * q + 6]), __uint_as_float(raw[8 * q + 7])));
+        }
+        sm.row_max[x][wg][r] = fmax3(mq[0], mq[1], fmaxf(mq[2], mq[3]));
+        // They are overwritten once S(x, j + 1) is there: its product follows P V(x, j), which every thread lets go
+        // only after the reads below.
         meet();
-        continue;
-      }
-      tc_fence_after();
-      uint32_t raw[kHalf];
-      tmem_ld32(s_addr, *reinterpret_cast<uint32_t(*)[32]>(&raw[0]));
-      tmem_ld32(s_addr + 32, *reinterpret_cast<uint32_t(*)[32]>(&raw[32]));
-      tmem_ld_wait();
-      const int left = lim - j * kBlock - half * kHalf;  // columns up to `left` are seen
-      if (left < kHalf - 1) {
+        const float m_tile = fmaxf(fmaxf(sm.row_max[x][0][r], sm.row_max[x][1][r]), fmaxf(sm.row_max[x][2][r], sm.row_max[x][3][r])) * sl2;
+        // The reference rises only when the tile's maximum exceeds it by more than 2^8: no exponential overflows,
+        // and after the first tiles of a row almost none has to be rescaled.
+        const bool raise = m_tile > m_ref[x] + kRescale;  // also the first visible tile (m_ref = -inf)
+        const float alpha = raise ? ex2_mufu(m_ref[x] - m_tile) : 1.0f;
+        if (raise) m_ref[x] = m_tile;
+        const float neg_m = (m_ref[x] == -INFINITY) ? 0.0f : -m_ref[x];
+        const unsigned long long s2 = f2_pack(sl2, sl2), nm2 = f2_pack(neg_m, neg_m);
+        unsigned long long sa = 0ull, sb = 0ull;  // pairs of partial sums
+        uint32_t pk[kCols / 2];
 #pragma unroll
-        for (int i = 0; i < kHalf; ++i) raw[i] = i > left ? 0xff800000u : raw[i];  // -inf
-      }
-      float mq[4];
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        mq[q] = fmax3(__uint_as_float(raw[q]), __uint_as_float(raw[q + 4]), __uint_as_float(raw[q + 8]));
-#pragma unroll
-        for (int i = q + 12; i + 4 < kHalf; i += 8) mq[q] = fmax3(mq[q], __uint_as_float(raw[i]), __uint_as_float(raw[i + 4]));
-        mq[q] = fmaxf(mq[q], __uint_as_float(raw[q + kHalf - 4]));
-      }
-      const float own = fmax3(mq[0], mq[1], fmaxf(mq[2], mq[3]));
-      sm.row_max[j & 1][x][half][r] = own;
-      meet();
-      const float m_tile = fmaxf(own, sm.row_max[j & 1][x][half ^ 1][r]) * sl2;
-      // The reference rises only when the tile's maximum exceeds it by more than 2^8: no exponential overflows,
-      // and after the first tiles of a row almost none has to be rescaled.
-      const float m_old = m_ref;
-      if (m_tile > m_ref + kRescale) m_ref = m_tile;  // also the first visible tile (m_ref = -inf)
-      const float neg_m = (m_ref == -INFINITY) ? 0.0f : -m_ref;
-      const unsigned long long s2 = f2_pack(sl2, sl2), nm2 = f2_pack(neg_m, neg_m);
-      unsigned long long sa = 0ull, sb = 0ull;  // pairs of partial sums
-#pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        uint32_t pk[16];
-#pragma unroll
-        for (int i = 0; i < 32; i += 2) {
+        for (int i = 0; i < kCols; i += 2) {
           float e0, e1;
-          f2_unpack(f2_fma(f2_pack(__uint_as_float(raw[c * 32 + i]), __uint_as_float(raw[c * 32 + i + 1])), s2, nm2), e0, e1);
-          if ((i & 7) == 6) {  // one pair of four on the FMA pipe, so that MUFU does not bound the tile
+          f2_unpack(f2_fma(f2_pack(__uint_as_float(raw[i]), __uint_as_float(raw[i + 1])), s2, nm2), e0, e1);
+          // part of the exponentials on the FMA pipe, so that MUFU does not bound the tile
+          if ((i & 7) == 6 || (kPolyEighths == 4 && (i & 7) == 2)) {
             exp2_poly2(e0, e1);
           } else {
             e0 = ex2_mufu(e0);
-            e1 = ex2_mufu(e1);
+            e1 = (kPolyEighths == 3 && (i & 7) == 2) ? exp2_poly(e1) : ex2_mufu(e1);
           }
           if (i & 2) sb = f2_add(sb, f2_pack(e0, e1));
           else sa = f2_add(sa, f2_pack(e0, e1));
           pk[i >> 1] = pack_bf16x2(e0, e1);
         }
-        tmem_st16(s_addr + c * 16, pk);
-      }
-      float s0, s1;
-      f2_unpack(f2_add(sa, sb), s0, s1);
-      const float alpha = (m_old == m_ref) ? 1.0f : ex2_mufu(m_old - m_ref);
-      l = l * alpha + (s0 + s1);
-      if (__any_sync(0xffffffffu, j > 0 && alpha != 1.0f)) {  // rare: O under an older reference, this half of its columns
+        tmem_st16(s_addr, pk);
+        float s0, s1;
+        f2_unpack(f2_add(sa, sb), s0, s1);
+        l[x] = l[x] * alpha + (s0 + s1);
+        if (__any_sync(0xffffffffu, raise && j > 0)) {  // rare: O under an older reference, this thread's columns
+          const uint32_t o_addr = tmem + lane_addr + O_COL(x) + wg * W;
 #pragma unroll
-        for (int c = 0; c < D / 2; c += 16) {
-          uint32_t ov[16];
-          tmem_ld16(o_addr + c, ov);
-          tmem_ld_wait();
+          for (int c = 0; c < W; c += 16) {
+            uint32_t ov[16];
+            tmem_ld16(o_addr + c, ov);
+            tmem_ld_wait();
 #pragma unroll
-          for (int i = 0; i < 16; ++i) ov[i] = __float_as_uint(__uint_as_float(ov[i]) * alpha);
-          tmem_st16(o_addr + c, ov);
-        }
-      }
-      // S(j) is there, so P V(j - 2) is done and this buffer's current or last phase is V(j)'s
-      if (clean && x == cleaner && j == n_max - 1) {
-        if (!mbar_wait_warp(&sm.v_full[j & 1], (j >> 1) & 1, p.status, kTimeoutFull)) {
-          ok = false;
-          continue;
-        }
-        clear_rows<D>(sm.v[j & 1], s.klen - j * kBlock, half * kBlock + r, 2 * kBlock);
-        fence_proxy_async();
-      }
-      tmem_st_wait();
-      tc_fence_before();
-      mbar_arrive(&sm.p_full[x]);
-    }
-    // ------------------------------------------------ O / l and the log-sum-exp
-    const bool row_ok = qi < s.qlen;
-    const long long row = s.q0 + qi;
-    __nv_bfloat16* orow = p.o + (row * p.Hq + h) * D + half * (D / 2);
-    if (n == 0) {
-      if (row_ok) {
-#pragma unroll
-        for (int c = 0; c < D / 16; ++c) reinterpret_cast<uint4*>(orow)[c] = make_uint4(0u, 0u, 0u, 0u);
-        if (p.lse != nullptr && half == 0) p.lse[static_cast<long long>(h) * p.pk.Nq + row] = -INFINITY;
-      }
-    } else {
-      if (ok) ok = mbar_wait_warp(&sm.o_done[x], (n - 1) & 1, p.status, kTimeoutAccFull);
-      // the last tile's maxima are in [(n - 1) & 1]: the sums go into the other buffer
-      sm.row_max[n & 1][x][half][r] = l;
-      meet();
-      if (ok) {
-        l += sm.row_max[n & 1][x][half ^ 1][r];
-        tc_fence_after();
-        const bool seen = lim >= 0;
-        const float inv_l = 1.0f / l;
-#pragma unroll
-        for (int c = 0; c < D / 2; c += 32) {
-          uint32_t ov[32];
-          tmem_ld32(o_addr + c, ov);
-          tmem_ld_wait();
-          if (row_ok) {
-            uint32_t w[16];
-#pragma unroll
-            for (int i = 0; i < 16; ++i)
-              w[i] = seen ? pack_bf16x2(__uint_as_float(ov[2 * i]) * inv_l, __uint_as_float(ov[2 * i + 1]) * inv_l) : 0u;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) reinterpret_cast<uint4*>(orow + c)[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+            for (int i = 0; i < 16; ++i) ov[i] = __float_as_uint(__uint_as_float(ov[i]) * alpha);
+            tmem_st16(o_addr + c, ov);
           }
         }
-        if (row_ok && half == 0 && p.lse != nullptr)
-          p.lse[static_cast<long long>(h) * p.pk.Nq + row] = seen ? (m_ref + log2f(l)) * 0.69314718055994531f : -INFINITY;
+        // S(j) is there, so P V(j - 2) is done and this buffer's current or last phase is V(j)'s
+        if (clean && x == cleaner && j == n_max - 1) {
+          if (!mbar_wait_warp(&sm.v_full[j & 1], (j >> 1) & 1, p.status, kTimeoutFull)) {
+            ok = false;
+            continue;
+          }
+          clear_rows<D>(sm.v[j & 1], s.klen - j * kBlock, wg * kBlock + r, kSoftmaxThreads);
+          fence_proxy_async();
+        }
+        tmem_st_wait();
+        tc_fence_before();
+        mbar_arrive(&sm.p_full[x]);
+      }
+    }
+    // ------------------------------------------------ O / l and the log-sum-exp
+    meet();  // the maxima have been read
+#pragma unroll
+    for (int x = 0; x < 2; ++x) sm.row_max[x][wg][r] = l[x];
+    meet();
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      const int qi = i0 + x * di + r;  // query within the sequence
+      const int h = h0 + x * dh;
+      const bool row_ok = qi < s.qlen;
+      const long long row = s.q0 + qi;
+      __nv_bfloat16* orow = p.o + (row * p.Hq + h) * D + wg * W;
+      const bool seen = min(qi + s.off, s.klen - 1) >= 0;
+      uint32_t w[W / 2];
+      if (n_x[x] == 0) {
+#pragma unroll
+        for (int i = 0; i < W / 2; ++i) w[i] = 0u;
+      } else {
+        if (!ok || !mbar_wait_warp(&sm.o_done[x], (n_x[x] - 1) & 1, p.status, kTimeoutAccFull)) break;
+        tc_fence_after();
+        const float sum = (sm.row_max[x][0][r] + sm.row_max[x][1][r]) + (sm.row_max[x][2][r] + sm.row_max[x][3][r]);
+        const float inv_l = 1.0f / sum;
+        uint32_t ov[W];
+        const uint32_t o_addr = tmem + lane_addr + O_COL(x) + wg * W;
+        if constexpr (W == 32) tmem_ld32(o_addr, ov);
+        else tmem_ld16(o_addr, ov);
+        tmem_ld_wait();
+#pragma unroll
+        for (int i = 0; i < W / 2; ++i)
+          w[i] = seen ? pack_bf16x2(__uint_as_float(ov[2 * i]) * inv_l, __uint_as_float(ov[2 * i + 1]) * inv_l) : 0u;
+        if (row_ok && wg == 0 && p.lse != nullptr)
+          p.lse[static_cast<long long>(h) * p.pk.Nq + row] = seen ? (m_ref[x] + log2f(sum)) * 0.69314718055994531f : -INFINITY;
+      }
+      if (row_ok) {
+#pragma unroll
+        for (int i = 0; i < W / 8; ++i) reinterpret_cast<uint4*>(orow)[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+        if (n_x[x] == 0 && wg == 0 && p.lse != nullptr) p.lse[static_cast<long long>(h) * p.pk.Nq + row] = -INFINITY;
       }
     }
   }
