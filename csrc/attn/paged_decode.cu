@@ -13,12 +13,12 @@
 // (sequence, head) last joins its partials in the order of the keys, so the result does not
 // depend on which CTA that was.
 //
-// Inside a CTA: K and V tiles stream through a ring of kStages buffers by 16-byte asynchronous
-// copies (rows found through the page table one tile ahead), and each of the four warps works on
-// 16 keys of a tile by itself: S = Q K^T and O += P V as 16x8x16 warp MMAs with the query heads
-// of the kv head as the rows (up to 16; tcgen05 needs 64 and would not move one byte faster), P
-// passing from accumulator to operand in registers.  The warps' softmax states meet once per
-// stretch, not per tile.
+// Inside a CTA: two producer warps stream K and V tiles through a ring of kStages buffers by 16-byte
+// asynchronous copies (half a warp per row of a head; pages looked up one tile ahead), so any page
+// size and order costs the same; and each of four consumer warps works on 16 keys of a tile by itself:
+// S = Q K^T and O += P V as 16x8x16 warp MMAs with the query heads of the kv head as the rows (up to
+// 16; tcgen05 needs 64 and would not move one byte faster), P passing from accumulator to operand in
+// registers.  The warps' softmax states meet once per stretch, not per tile.
 #include "common/host_utils.h"
 #include "common/ptx.cuh"
 #include "common/fast_exp2.cuh"
@@ -29,8 +29,10 @@ namespace tt {
 namespace paged {
 
 constexpr int kTile = 64;      // keys per unit
-constexpr int kThreads = 128;  // 4 warps x 16 keys
-constexpr int kWarps = kThreads / 32;
+constexpr int kWarps = 4;       // consumer warps, 16 keys each
+constexpr int kProducers = 64;  // threads of the two producer warps, 32 keys each
+constexpr int kThreads = kWarps * 32 + kProducers;
+constexpr int kAllWarps = kThreads / 32;
 constexpr int kStages = 3;
 constexpr int kCtasPerSm = 2;
 constexpr int kMaxG = 16;      // query heads per kv head
@@ -57,11 +59,13 @@ struct Params {
 __device__ __forceinline__ void cp_async16(uint32_t smem, const void* gmem, bool valid) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem), "l"(gmem), "r"(valid ? 16 : 0) : "memory");
 }
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_async_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+// Arrive on the barrier when this thread's copies so far have landed (counted in the barrier's expected arrivals).
+__device__ __forceinline__ void cp_async_arrive(uint64_t* bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
+__device__ __forceinline__ void cp_async_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+__device__ __forceinline__ void consumers_meet() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
+static_assert(kWarps * 32 == 128, "the consumers' barrier");
 __device__ __forceinline__ void ldsm_x4(uint32_t (&r)[4], uint32_t addr) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
@@ -84,9 +88,9 @@ template <int D>
 struct Smem {
   alignas(128) uint8_t k[kStages][kTile * D * 2];
   alignas(128) uint8_t v[kStages][kTile * D * 2];
-  int rows[kStages + 1][kTile];     // pool row of each key of a tile (-1: none)
   float m[kWarps][kMaxG], l[kWarps][kMaxG];
-  int scan[kWarps];
+  uint64_t full[kStages], empty[kStages];
+  int scan[kAllWarps];
   int find[3];
   int last;
 };
@@ -105,19 +109,41 @@ __device__ __forceinline__ int seq_len(const Params& p, int b) {
   return n < 0 ? 0 : static_cast<int>(min(static_cast<long long>(n), most));
 }
 
+// Inclusive scan over the block's threads within their warp; base: the sum of the warps before, sum: of all.
+__device__ __forceinline__ int block_scan(int n, int lane, int warp, int* scratch, int& base, int& sum) {
+  int incl = n;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int up = __shfl_up_sync(0xffffffffu, incl, o);
+    if (lane >= o) incl += up;
+  }
+  if (lane == 31) scratch[warp] = incl;
+  __syncthreads();
+  base = 0;
+  sum = 0;
+#pragma unroll
+  for (int w = 0; w < kAllWarps; ++w) {
+    if (w < warp) base += scratch[w];
+    sum += scratch[w];
+  }
+  __syncthreads();
+  return incl;
+}
+
 template <int D>
 __global__ void __launch_bounds__(kThreads, kCtasPerSm) paged_decode_kernel(const Params p) {
   static_assert(D == 64 || D == 128, "head_dim 64 or 128");
   constexpr int NU = D / 8;          // 16-byte units per row
   constexpr int KS = D / 16;         // MMA k-steps of Q K^T
-  constexpr int ROWS_PER_PASS = kThreads / NU;
   extern __shared__ __align__(128) uint8_t smem_raw[];
   Smem<D>& sm = *reinterpret_cast<Smem<D>*>(smem_raw);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int cta = blockIdx.x;
 
-  // ---- the line of units: its length, and where this CTA's stretch begins
-  long long total_tiles = 0;  // tiles per kv head over all sequences
+  // ---- the line of units: its length, and where this CTA's stretch begins.  One scan where a step of it holds
+  // all sequences, a second one over the steps otherwise.
+  int n_first = 0, incl_first = 0;  // of this thread's sequence in the first step
+  long long total_tiles = 0;        // tiles per kv head over all sequences
   for (int b0 = 0; b0 < p.B; b0 += kThreads) {
     const int b = b0 + tid;
     int n = 0;
@@ -130,13 +156,13 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) paged_decode_kernel(cons
         for (int i = 0; i < p.Hq * NU; ++i) o[i] = make_uint4(0u, 0u, 0u, 0u);
       }
     }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
-    if (lane == 0) sm.scan[warp] = n;
-    __syncthreads();
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) total_tiles += sm.scan[w];
-    __syncthreads();
+    int base, sum;
+    const int incl = block_scan(n, lane, warp, sm.scan, base, sum) + base;
+    if (b0 == 0) {
+      n_first = n;
+      incl_first = incl;
+    }
+    total_tiles += sum;
   }
   const long long W = total_tiles * p.Hkv;
   const int ctas = static_cast<int>(min(static_cast<long long>(gridDim.x), W));  // each has a unit at least
@@ -146,22 +172,14 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) paged_decode_kernel(cons
     long long before = 0;  // units of the sequences before b0
     for (int b0 = 0; b0 < p.B; b0 += kThreads) {
       const int b = b0 + tid;
-      const int n = b < p.B ? (seq_len(p, b) + kTile - 1) / kTile : 0;
-      int incl = n;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int up = __shfl_up_sync(0xffffffffu, incl, o);
-        if (lane >= o) incl += up;
+      int n = n_first, incl = incl_first, base, sum = 0;
+      if (b0 > 0) {
+        n = b < p.B ? (seq_len(p, b) + kTile - 1) / kTile : 0;
+        incl = block_scan(n, lane, warp, sm.scan, base, sum) + base;
+      } else if (p.B > kThreads) {
+        block_scan(n, lane, warp, sm.scan, base, sum);
       }
-      if (lane == 31) sm.scan[warp] = incl;
-      __syncthreads();
-      int base = 0, sum = 0;
-#pragma unroll
-      for (int w = 0; w < kWarps; ++w) {
-        if (w < warp) base += sm.scan[w];
-        sum += sm.scan[w];
-      }
-      const long long first = before + static_cast<long long>(base + incl - n) * p.Hkv;
+      const long long first = before + static_cast<long long>(incl - n) * p.Hkv;
       const long long end = first + static_cast<long long>(n) * p.Hkv;
       if (n > 0 && first <= u0 && u0 < end) {
         const int r = static_cast<int>(u0 - first);
@@ -170,78 +188,72 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) paged_decode_kernel(cons
         sm.find[2] = r % n;
       }
       before += static_cast<long long>(sum) * p.Hkv;
-      __syncthreads();
       if (before > u0) break;
     }
   }
+  if (tid == 0) {
+    for (int i = 0; i < kStages; ++i) {
+      mbar_init(&sm.full[i], kProducers);
+      mbar_init(&sm.empty[i], kWarps);
+    }
+    fence_barrier_init();
+  }
+  __syncthreads();
   int b = sm.find[0], kvh = sm.find[1], tile = sm.find[2];
   int len = seq_len(p, b), n_tiles = (len + kTile - 1) / kTile;
 
-  // ---- loads run kStages - 1 tiles ahead of the math; (lb, lh, lt) is the next tile whose rows are
-  // looked up, one tile ahead of its loads
-  int lb = b, lh = kvh, lt = tile, llen = len;
   const int count = static_cast<int>(u1 - u0);
-  int ahead = 0;  // tiles whose rows have been looked up
-  auto look_up = [&]() {
-    if (ahead < count) {
-      if (tid < kTile) {
-        const int key = lt * kTile + tid;
-        int row = -1;
-        if (key < llen) {
-          const int page = p.table[static_cast<long long>(lb) * p.width + key / p.page_size];
-          if (page >= 0 && page < p.num_pages) row = page * p.page_size + key % p.page_size;
-          else atomicCAS(p.status, 0, static_cast<int>(kBadIndex));
-        }
-        sm.rows[ahead % (kStages + 1)][tid] = row;
-      }
-      ++ahead;
-      if (++lt * kTile >= llen) {
-        lt = 0;
-        if (++lh == p.Hkv) {
-          lh = 0;
-          if (ahead < count) {
-            do { ++lb; llen = seq_len(p, lb); } while (llen == 0);
-          }
-        }
-      }
-    }
-  };
-  int fh = kvh, fb = b, ft = tile, flen = len;  // the next tile to be fetched
-  int fetched = 0;
   const uint32_t k_base = smem_u32(sm.k[0]), v_base = smem_u32(sm.v[0]);
   constexpr uint32_t STAGE = kTile * D * 2;
-  auto fetch = [&]() {
-    if (fetched < count) {
-      const int s = fetched % kStages;
-      const int* rows = sm.rows[fetched % (kStages + 1)];
-      const int u = tid % NU;
-#pragma unroll
-      for (int j = 0; j < kTile / ROWS_PER_PASS; ++j) {
-        const int r = j * ROWS_PER_PASS + tid / NU;
-        const int row = rows[r];
-        const long long off = row >= 0 ? (static_cast<long long>(row) * p.Hkv + fh) * D + 8 * u : 0;
-        cp_async16(k_base + s * STAGE + unit_off<D>(r, u), p.k_pages + off, row >= 0);
-        cp_async16(v_base + s * STAGE + unit_off<D>(r, u), p.v_pages + off, row >= 0);
+
+  if (warp >= kWarps) {
+    // ---------------------------------------------------------------- producers: keys [32 w, 32 w + 32) of every tile
+    const int row0 = (warp - kWarps) * 32;
+    int page = -1, off = -1;  // of this lane's key of tile (b, tile); off < 0: no key
+    auto look_up = [&]() {
+      const int key = tile * kTile + row0 + lane;
+      page = -1;
+      off = -1;
+      if (key < len) {
+        const int pi = key / p.page_size;
+        off = key - pi * p.page_size;
+        page = p.table[static_cast<long long>(b) * p.width + pi];
       }
-      ++fetched;
-      if (++ft * kTile >= flen) {
-        ft = 0;
-        if (++fh == p.Hkv) {
-          fh = 0;
-          if (fetched < count) {
-            do { ++fb; flen = seq_len(p, fb); } while (flen == 0);
+    };
+    look_up();
+    for (int i = 0; i < count; ++i) {
+      const bool mapped = page >= 0 && page < p.num_pages;
+      if (off >= 0 && !mapped) atomicCAS(p.status, 0, static_cast<int>(kBadIndex));
+      const int row = off >= 0 && mapped ? page * p.page_size + off : -1;
+      const int head = kvh;
+      if (++tile * kTile >= len) {  // the tile after this one
+        tile = 0;
+        if (++kvh == p.Hkv) {
+          kvh = 0;
+          if (i + 1 < count) {
+            do { ++b; len = seq_len(p, b); } while (len == 0);
           }
         }
       }
+      if (i + 1 < count) look_up();  // its latency lies beside this tile's copies
+      const int st = i % kStages;
+      if (!mbar_wait_warp(&sm.empty[st], ((i / kStages) & 1) ^ 1u, p.status, kTimeoutEmpty)) break;
+      const int u = lane % NU;
+#pragma unroll 4
+      for (int j = 0; j < NU; ++j) {  // 32 / NU rows of a head at a time
+        const int r = j * (32 / NU) + lane / NU;
+        const int from = __shfl_sync(0xffffffffu, row, r);
+        const long long at = from >= 0 ? (static_cast<long long>(from) * p.Hkv + head) * D + 8 * u : 0;
+        const uint32_t to = st * STAGE + unit_off<D>(row0 + r, u);
+        cp_async16(k_base + to, p.k_pages + at, from >= 0);
+        cp_async16(v_base + to, p.v_pages + at, from >= 0);
+      }
+      cp_async_arrive(&sm.full[st]);
     }
-    cp_async_commit();
-  };
-#pragma unroll
-  for (int i = 0; i < kStages; ++i) look_up();
-  __syncthreads();
-#pragma unroll
-  for (int i = 0; i < kStages - 1; ++i) fetch();
-
+    cp_async_wait_all();
+    return;
+  }
+  // ------------------------------------------------------------------ consumers
   const int g = lane >> 2, c2 = 2 * (lane & 3);  // accumulator row (and g + 8), column pair
   const int lr = lane & 7, lm = lane >> 3;       // ldmatrix: row in a matrix, matrix
   int done = 0;
@@ -269,14 +281,11 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) paged_decode_kernel(cons
       for (int j = 0; j < 4; ++j) o[i][j] = 0.0f;
     float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.0f, l1 = 0.0f;  // rows g, g + 8 of this warp's keys
     for (int it = 0; it < seg_tiles; ++it, ++done, ++tile) {
-      cp_async_wait<kStages - 2>();
-      __syncthreads();  // the tile has landed for all threads, and the buffer fetched next is no longer read
-      fetch();
-      look_up();
       const int s = done % kStages;
+      if (!mbar_wait_warp(&sm.full[s], (done / kStages) & 1, p.status, kTimeoutFull)) continue;  // and the next, and the end
       const uint32_t kb = k_base + s * STAGE, vb = v_base + s * STAGE;
       const int key0 = tile * kTile + warp * 16;
-      if (key0 >= len) continue;  // none of this warp's keys
+      if (key0 < len) {  // else none of this warp's keys
       float sc[2][4] = {};
 #pragma unroll
       for (int k = 0; k < KS; ++k) {
@@ -335,6 +344,9 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) paged_decode_kernel(cons
         mma_16816(o[i], pa, bv[0], bv[1]);
         mma_16816(o[i + 1], pa, bv[2], bv[3]);
       }
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sm.empty[s]);
     }
     // ---- the four warps' states of this (sequence, head) into one
 #pragma unroll
@@ -348,7 +360,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) paged_decode_kernel(cons
       sm.l[warp][g] = l0;
       sm.l[warp][g + 8] = l1;
     }
-    __syncthreads();
+    consumers_meet();
     float M0 = sm.m[0][g], M1 = sm.m[0][g + 8];
 #pragma unroll
     for (int w = 1; w < kWarps; ++w) {
@@ -370,12 +382,12 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) paged_decode_kernel(cons
           *a1 = make_float2(x1.x + f1 * o[i][2], x1.y + f1 * o[i][3]);
         }
       }
-      __syncthreads();
+      consumers_meet();
     }
     const bool whole = seg_tile0 == 0 && seg_tiles == n_tiles;
     const long long pair = static_cast<long long>(b) * p.Hkv + kvh;
     if (whole) {
-      for (int i = tid; i < p.G * D / 2; i += kThreads) {
+      for (int i = tid; i < p.G * D / 2; i += kWarps * 32) {
         const int h = i / (D / 2), d = 2 * (i % (D / 2));
         float M = sm.m[0][h], L = 0.0f;
 #pragma unroll
@@ -387,7 +399,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) paged_decode_kernel(cons
       }
     } else {
       const long long slot = 2ll * cta + seg;
-      for (int i = tid; i < p.G * D / 4; i += kThreads)
+      for (int i = tid; i < p.G * D / 4; i += kWarps * 32)
         reinterpret_cast<float4*>(p.part_o + slot * p.G * D)[i] = reinterpret_cast<const float4*>(acc)[i];
       if (tid < p.G) {
         float M = sm.m[0][tid], L = 0.0f;
@@ -402,34 +414,61 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) paged_decode_kernel(cons
       const long long first = u0 + done - (seg_tile0 + seg_tiles), end = first + n_tiles;
       const int ca = static_cast<int>(((first + 1) * ctas - 1) / W), cb = static_cast<int>((end * ctas - 1) / W);
       __threadfence();
-      __syncthreads();
+      consumers_meet();
       if (tid == 0) sm.last = atomicAdd(p.counters + pair, 1) == cb - ca ? 1 : 0;
-      __syncthreads();
+      consumers_meet();
       if (sm.last) {  // all partials are there: join them in key order
         __threadfence();
         if (tid == 0) p.counters[pair] = 0;
         // A CTA's partial of this pair is its first one unless the pair began inside its stretch.
-        auto slot_of = [&](int c) { return 2ll * c + ((c == ca && W * c / ctas < first) ? 1 : 0); };
-        for (int i = tid; i < p.G * D / 2; i += kThreads) {
-          const int h = i / (D / 2), d = 2 * (i % (D / 2));
-          float M = -INFINITY;
-          for (int c = ca; c <= cb; ++c) M = fmaxf(M, __ldcg(p.part_ml + (slot_of(c) * p.G + h) * 2));
-          float L = 0.0f, x = 0.0f, y = 0.0f;
-          for (int c = ca; c <= cb; ++c) {
-            const long long sl = slot_of(c) * p.G + h;
-            const float2 ml = __ldcg(reinterpret_cast<const float2*>(p.part_ml + sl * 2));
-            const float2 v = __ldcg(reinterpret_cast<const float2*>(p.part_o + sl * D + d));
-            const float f = ml.x == -INFINITY ? 0.0f : ex2_mufu(ml.x - M);
-            L = fmaf(f, ml.y, L);
-            x = fmaf(f, v.x, x);
-            y = fmaf(f, v.y, y);
+        auto slot_of = [&](int c) { return (2ll * c + ((c == ca && W * c / ctas < first) ? 1 : 0)) * p.G; };
+        for (int h = warp; h < p.G; h += kWarps) {  // the heads' maxima and sums, lanes over the partials
+          float M = -INFINITY, L = 0.0f;
+          for (int c = ca + lane; c <= cb; c += 32) M = fmaxf(M, __ldcg(p.part_ml + (slot_of(c) + h) * 2));
+#pragma unroll
+          for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+          for (int c = ca + lane; c <= cb; c += 32) {
+            const float2 ml = __ldcg(reinterpret_cast<const float2*>(p.part_ml + (slot_of(c) + h) * 2));
+            if (ml.x != -INFINITY) L = fmaf(ex2_mufu(ml.x - M), ml.y, L);
           }
-          const float inv = 1.0f / L;
-          *reinterpret_cast<uint32_t*>(p.out + (pair * p.G + h) * D + d) = pack_bf16x2(x * inv, y * inv);
+#pragma unroll
+          for (int o = 16; o > 0; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
+          if (lane == 0) {
+            sm.m[0][h] = M;
+            sm.l[0][h] = 1.0f / L;
+          }
+        }
+        consumers_meet();
+        for (int i = tid; i < p.G * D / 4; i += kWarps * 32) {
+          const int h = i / (D / 4), d = 4 * (i % (D / 4));
+          const float M = sm.m[0][h];
+          float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+          constexpr int kBatch = 8;  // partials loaded at once
+          for (int c0 = ca; c0 <= cb; c0 += kBatch) {
+            float f[kBatch];
+            float4 v[kBatch];
+#pragma unroll
+            for (int n = 0; n < kBatch; ++n) {
+              const long long sl = slot_of(min(c0 + n, cb)) + h;
+              f[n] = __ldcg(p.part_ml + sl * 2);
+              v[n] = __ldcg(reinterpret_cast<const float4*>(p.part_o + sl * D + d));
+            }
+#pragma unroll
+            for (int n = 0; n < kBatch; ++n) {
+              const float w = (c0 + n > cb || f[n] == -INFINITY) ? 0.0f : ex2_mufu(f[n] - M);
+              x.x = fmaf(w, v[n].x, x.x);
+              x.y = fmaf(w, v[n].y, x.y);
+              x.z = fmaf(w, v[n].z, x.z);
+              x.w = fmaf(w, v[n].w, x.w);
+            }
+          }
+          const float inv = sm.l[0][h];
+          *reinterpret_cast<uint2*>(p.out + (pair * p.G + h) * D + d) =
+              make_uint2(pack_bf16x2(x.x * inv, x.y * inv), pack_bf16x2(x.z * inv, x.w * inv));
         }
       }
     }
-    __syncthreads();  // acc, m and l are free again
+    consumers_meet();  // acc, m and l are free again
     seg = 1;
     if (tile == n_tiles) {
       tile = 0;
@@ -442,7 +481,6 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) paged_decode_kernel(cons
       }
     }
   }
-  cp_async_wait<0>();
 }
 
 template <int D>
