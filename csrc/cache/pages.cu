@@ -85,15 +85,23 @@ __global__ void __launch_bounds__(kThreads) rotary_append_kernel(const AppendArg
   const int rot = (a.Hq + a.Hkv) * groups;
   const float* cr = a.cos_t + static_cast<long long>(pos) * half;
   const float* sr = a.sin_t + static_cast<long long>(pos) * half;
-#pragma unroll 4
-  for (int i = lane; i < rot; i += 32) {
+  // A lane keeps its piece of the head where the pieces of a head divide the warp (D = 16 to 256 in powers of two):
+  // the angles are then loaded once.
+  const bool same_piece = 32 % groups == 0;
+  float cs[8], sn[8];
+  auto angles = [&](int d0) {
+    const float4 ca = *reinterpret_cast<const float4*>(cr + d0), cb = *reinterpret_cast<const float4*>(cr + d0 + 4);
+    const float4 sa = *reinterpret_cast<const float4*>(sr + d0), sb = *reinterpret_cast<const float4*>(sr + d0 + 4);
+    cs[0] = ca.x, cs[1] = ca.y, cs[2] = ca.z, cs[3] = ca.w, cs[4] = cb.x, cs[5] = cb.y, cs[6] = cb.z, cs[7] = cb.w;
+    sn[0] = sa.x, sn[1] = sa.y, sn[2] = sa.z, sn[3] = sa.w, sn[4] = sb.x, sn[5] = sb.y, sn[6] = sb.z, sn[7] = sb.w;
+  };
+  if (same_piece) angles(8 * (lane % groups));
+#pragma unroll 2
+  for (int i = lane; i < rot; i += 32) {  // a lane reads both halves of a piece before it writes them (the output may be the input)
     const int h = i / groups, d0 = 8 * (i - h * groups);
     const uint4 lo4 = *reinterpret_cast<const uint4*>(src + h * a.D + d0);
     const uint4 hi4 = *reinterpret_cast<const uint4*>(src + h * a.D + half + d0);
-    const float4 ca = *reinterpret_cast<const float4*>(cr + d0), cb = *reinterpret_cast<const float4*>(cr + d0 + 4);
-    const float4 sa = *reinterpret_cast<const float4*>(sr + d0), sb = *reinterpret_cast<const float4*>(sr + d0 + 4);
-    const float cs[8] = {ca.x, ca.y, ca.z, ca.w, cb.x, cb.y, cb.z, cb.w};
-    const float sn[8] = {sa.x, sa.y, sa.z, sa.w, sb.x, sb.y, sb.z, sb.w};
+    if (!same_piece) angles(d0);
     const uint32_t* lw = reinterpret_cast<const uint32_t*>(&lo4);
     const uint32_t* hw = reinterpret_cast<const uint32_t*>(&hi4);
     uint4 olo, ohi;
@@ -153,16 +161,21 @@ struct CopyArgs {
 
 constexpr int kInFlight = 8;  // 16-byte loads a thread keeps in flight
 
+// kOnce: the source is read by this copy alone (a fork's source by every child of a parent).
+template <bool kOnce>
 __device__ __forceinline__ void copy_vecs(uint4* dst, const uint4* src, int n) {
-  int i = threadIdx.x;
-  for (; i + (kInFlight - 1) * kThreads < n; i += kInFlight * kThreads) {
+  for (int i = threadIdx.x; i < n; i += kInFlight * kThreads) {
     uint4 r[kInFlight];
 #pragma unroll
-    for (int j = 0; j < kInFlight; ++j) r[j] = src[i + j * kThreads];
+    for (int j = 0; j < kInFlight; ++j)
+      if (i + j * kThreads < n) r[j] = kOnce ? __ldcs(src + i + j * kThreads) : src[i + j * kThreads];
 #pragma unroll
-    for (int j = 0; j < kInFlight; ++j) dst[i + j * kThreads] = r[j];
+    for (int j = 0; j < kInFlight; ++j)
+      if (i + j * kThreads < n) {
+        if (kOnce) __stcs(dst + i + j * kThreads, r[j]);
+        else dst[i + j * kThreads] = r[j];
+      }
   }
-  for (; i < n; i += kThreads) dst[i] = src[i];
 }
 
 __device__ __forceinline__ void bad_index(int* status) {
@@ -170,6 +183,7 @@ __device__ __forceinline__ void bad_index(int* status) {
 }
 
 // Data block `blk`: copy number, layer, k or v, piece of the page.
+template <bool kOnce>
 __device__ __forceinline__ void copy_page_piece(const CopyArgs& a, long long blk, int src, int dst) {
   const int piece = static_cast<int>(blk % a.chunks);
   const long long rest = blk / a.chunks;
@@ -178,7 +192,7 @@ __device__ __forceinline__ void copy_page_piece(const CopyArgs& a, long long blk
   uint4* pool = which ? a.v : a.k;
   const long long base = static_cast<long long>(layer) * a.num_pages;
   const int off = piece * a.chunk;
-  copy_vecs(pool + (base + dst) * a.page_vecs + off, pool + (base + src) * a.page_vecs + off, min(a.chunk, a.page_vecs - off));
+  copy_vecs<kOnce>(pool + (base + dst) * a.page_vecs + off, pool + (base + src) * a.page_vecs + off, min(a.chunk, a.page_vecs - off));
 }
 
 // Child c_i takes the row and length of parent p_i; where fresh f_i >= 0, the parent's page that
@@ -205,7 +219,7 @@ __global__ void __launch_bounds__(kThreads) fork_kernel(const CopyArgs a) {
       bad_index(a.status);
       return;
     }
-    copy_page_piece(a, blk, src, fresh);
+    copy_page_piece<false>(a, blk, src, fresh);
     return;
   }
   const int* from = a.table + static_cast<long long>(parent) * a.width;
@@ -225,7 +239,7 @@ __global__ void __launch_bounds__(kThreads) move_kernel(const CopyArgs a) {
       bad_index(a.status);
       return;
     }
-    copy_page_piece(a, blk, src, dst);
+    copy_page_piece<true>(a, blk, src, dst);
     return;
   }
   const long long e = (blk - a.data_blocks) * kThreads + threadIdx.x;

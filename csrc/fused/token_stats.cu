@@ -6,12 +6,15 @@
 //   entropy   = -sum p log p = log s - u / s
 //   top i     = the i-th largest x (ties: lowest index first), log p = d - log s
 //   d/dx_j    = g_lp (1[j = t] - p_j) - g_ent p_j (log p_j + H) + sum_i g_i (1[j = id_i] - p_j)
-// Subtracting the maximum before anything is multiplied keeps entropy and log-probs exact to
-// fp32 rounding whatever the offset of the logits; (m, log s) are kept apart for the backward
-// for the same reason (their sum would round away bits of log s at large m).
+// (m, log s) are kept apart for the backward: their sum would round away bits of log s at large m.
 //
-// Forward: one pass.  A thread keeps (m, s, u) of its elements and raises m only when a
-// 16-byte vector holds a larger value.  The alternatives ride along without a second pass over
+// Forward: one pass, in the log2 domain about c = fl(m log2e).  One FMA forms y_j = x_j log2e - c, so
+// s' = sum 2^y and u' = sum 2^y y share one offset delta = m log2e - c (known exactly from another FMA):
+// entropy = ln2 (log2 s' - u' / s') does not depend on it, log s = ln2 (log2 s' - delta).  An element
+// costs an FMA, an exponential, an add and an FMA; with about 8 cycles a warp the exponential (MUFU) is
+// the most of it, 16 elements a cycle and SM, against 11.6 that memory delivers.  A thread keeps (m, s', u')
+// of its elements and raises m only when a 16-byte vector holds a larger value.  Values below -1e6 (masked
+// tokens) count as -1e6 there; a row with nothing above that is done again exactly.  The alternatives ride along without a second pass over
 // the row: the k-th largest of the 32 half-warp maxima bounds the k-th largest element from
 // below, so only threads whose own maximum reaches that bound look at their elements again
 // (about k of them), and the few candidates are ranked in shared memory.
@@ -28,6 +31,7 @@ constexpr int kGroups = 32;    // half-warp maxima that bound the k-th largest e
 constexpr int kMaxTop = 32;
 constexpr int kMaxCand = 512;  // candidates ranked in shared memory; more (mass ties): the slow path
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
 static_assert(kThreads / 16 == kGroups && kMaxTop <= kGroups, "one bound per half warp");
 
 template <typename T>
@@ -48,6 +52,20 @@ struct Elem<__nv_bfloat16> {
     return make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
   }
   __device__ static __nv_bfloat16 round(float x) { return __float2bfloat16_rn(x); }
+  // Values of a vector, those below the floor raised to it (a NaN stays), and the largest (NaN left out).
+  __device__ static float floored(const uint4& q, float (&v)[8]) {
+    constexpr uint32_t kLow = 0xc974c974u;  // bf16 pair of -999424
+    uint32_t w[4] = {q.x, q.y, q.z, q.w};
+    uint32_t m;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) asm("max.NaN.bf16x2 %0, %0, %1;" : "+r"(w[i]) : "r"(kLow));
+    uint32_t a, b;
+    asm("max.bf16x2 %0, %1, %2;" : "=r"(a) : "r"(w[0]), "r"(w[1]));
+    asm("max.bf16x2 %0, %1, %2;" : "=r"(b) : "r"(w[2]), "r"(w[3]));
+    asm("max.bf16x2 %0, %1, %2;" : "=r"(m) : "r"(a), "r"(b));
+    unpack(make_uint4(w[0], w[1], w[2], w[3]), v);
+    return fmaxf(__uint_as_float(m << 16), __uint_as_float(m & 0xffff0000u));
+  }
 };
 template <>
 struct Elem<float> {
@@ -63,6 +81,16 @@ struct Elem<float> {
     return make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
   }
   __device__ static float round(float x) { return x; }
+  __device__ static float floored(const uint4& q, float (&v)[4]) {
+    unpack(q, v);
+    float m = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      asm("max.NaN.f32 %0, %0, %1;" : "+f"(v[i]) : "f"(-1e6f));
+      m = fmaxf(m, v[i]);
+    }
+    return m;
+  }
 };
 
 // Order of the values as unsigned integers: NaN lowest (0), then -inf .. +inf; -0 equals +0.
@@ -82,20 +110,55 @@ __device__ __forceinline__ float max_nan(float a, float b) {  // NaN if either i
   return r;
 }
 
+constexpr float kFloor = -1e6f;  // what lower values count as in the first pass
+constexpr float kFar = 9e5f;     // a row whose maximum is further from zero is summed again exactly (c would round too much)
+
 struct Acc {
-  float m = -INFINITY, s = 0.0f, u = 0.0f;
-  __device__ __forceinline__ void raise(float m2) {  // m2 > m
-    if (m != -INFINITY) {
-      const float dm = m - m2;
-      const float c = ex2_mufu(dm * kLog2e);
-      u = c * fmaf(dm, s, u);
-      s *= c;
-      if (c == 0.0f) u = 0.0f;  // dm may be -inf
-    }
-    m = m2;
+  float m = -INFINITY, c = 0.0f, s = 0.0f, u = 0.0f;
+  // Moves the sums from reference `from` to a larger one.
+  __device__ __forceinline__ void shift(float from, float to) {
+    const float dc = from - to;
+    const float f = ex2_mufu(dc);
+    u = f == 0.0f ? 0.0f : f * fmaf(dc, s, u);  // dc may be -inf
+    s *= f;                                     // a NaN of s stays
   }
-  // Adds elements whose maximum has been raised into m.  The floor keeps 0 * -inf out of u for
-  // elements of -inf (or of the type's lowest value, masked tokens); a NaN passes through.
+  __device__ __forceinline__ void raise(float m2) {  // m2 > m
+    const float c2 = m2 * kLog2e;
+    if (m != -INFINITY) shift(c, c2);
+    m = m2;
+    c = c2;
+  }
+  template <int N>
+  __device__ __forceinline__ void add(const float (&v)[N]) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const float y = fmaf(v[i], kLog2e, -c);
+      const float e = ex2_mufu(y);
+      s += e;
+      u = fmaf(e, y, u);
+    }
+  }
+  __device__ __forceinline__ void merge(float m2, float s2, float u2) {
+    float c2 = m2 == -INFINITY ? 0.0f : m2 * kLog2e;
+    if (m2 > m) {
+      const float a = m, d = c, x = s, y = u;
+      m = m2, c = c2, s = s2, u = u2;
+      m2 = a, c2 = d, s2 = x, u2 = y;
+    }
+    if (m2 != -INFINITY) {
+      const float dc = c2 - c;
+      const float f = ex2_mufu(dc);
+      s += f * s2;
+      if (f != 0.0f) u += f * fmaf(dc, s2, u2);
+    } else {
+      s += s2;  // zero, or the NaN of elements that have no maximum
+    }
+  }
+};
+
+// The same sums in natural units about a known maximum, for rows of only masked tokens.
+struct AccExact {
+  float m = -INFINITY, s = 0.0f, u = 0.0f;
   template <int N>
   __device__ __forceinline__ void add(const float (&v)[N]) {
     const float mm = m == -INFINITY ? 0.0f : m;
@@ -107,22 +170,28 @@ struct Acc {
       u = fmaf(e, d, u);
     }
   }
-  __device__ __forceinline__ void merge(float m2, float s2, float u2) {
-    if (m2 > m) {
-      const float a = m, b = s, c = u;
-      m = m2, s = s2, u = u2;
-      m2 = a, s2 = b, u2 = c;
-    }
-    if (m2 != -INFINITY) {
-      const float dm = m2 - m;
-      const float c = ex2_mufu(dm * kLog2e);
-      s += c * s2;                                   // a NaN of s2 stays even where c is 0
-      if (c != 0.0f) u += c * fmaf(dm, s2, u2);      // dm s2 may overflow there
-    } else {
-      s += s2;  // zero, or the NaN of elements that have no maximum
-    }
-  }
 };
+
+__device__ __forceinline__ float block_sum(float v, float* scratch, int lane, int warp) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  __syncthreads();
+  if (lane == 0) scratch[warp] = v;
+  __syncthreads();
+  v = 0.0f;
+  for (int w = 0; w < kThreads / 32; ++w) v += scratch[w];
+  return v;
+}
+__device__ __forceinline__ float block_max(float v, float* scratch, int lane, int warp) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+  __syncthreads();
+  if (lane == 0) scratch[warp] = v;
+  __syncthreads();
+  v = scratch[0];
+  for (int w = 1; w < kThreads / 32; ++w) v = fmaxf(v, scratch[w]);
+  return v;
+}
 
 struct FwdArgs {
   const void* logits;
@@ -164,6 +233,7 @@ __global__ void __launch_bounds__(kThreads) token_stats_fwd_kernel(const FwdArgs
   __shared__ unsigned long long best[kThreads / 32];
   __shared__ int n_cand;
   __shared__ uint32_t bound_s;
+  __shared__ float total[3];
   const int row = blockIdx.x;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int64_t t = a.targets[row];
@@ -188,10 +258,7 @@ __global__ void __launch_bounds__(kThreads) token_stats_fwd_kernel(const FwdArgs
   Acc acc;
   auto take = [&](const uint4& q) {
     float v[kVec];
-    Elem<T>::unpack(q, v);
-    float vm = v[0];
-#pragma unroll
-    for (int i = 1; i < kVec; ++i) vm = fmaxf(vm, v[i]);
+    const float vm = Elem<T>::floored(q, v);
     if (vm > acc.m) acc.raise(vm);
     acc.add(v);
   };
@@ -208,7 +275,7 @@ __global__ void __launch_bounds__(kThreads) token_stats_fwd_kernel(const FwdArgs
   const int edge = tid < rs.head ? tid : (tid - rs.head + tail);
   const bool has_edge = edge < a.V && (tid < rs.head || tid - rs.head < a.V - tail);
   if (has_edge) {
-    const float v[1] = {Elem<T>::one(x + edge)};
+    const float v[1] = {max_nan(Elem<T>::one(x + edge), kFloor)};
     if (v[0] > acc.m) acc.raise(v[0]);
     acc.add(v);
   }
@@ -232,27 +299,67 @@ __global__ void __launch_bounds__(kThreads) token_stats_fwd_kernel(const FwdArgs
     red[2][warp] = acc.u;
   }
   __syncthreads();
-  Acc all;  // every thread, in warp order: the same sum in all of them
-  for (int w = 0; w < kThreads / 32; ++w) all.merge(red[0][w], red[1][w], red[2][w]);
-  const float log_s = all.m == -INFINITY ? NAN : logf(all.s);  // nothing above -inf: 0 / 0
+  if (warp == 0) {  // the warps' sums, in the order of a fixed tree
+    Acc w;
+    if (lane < kThreads / 32) w.merge(red[0][lane], red[1][lane], red[2][lane]);
+#pragma unroll
+    for (int o = kThreads / 64; o > 0; o >>= 1) {
+      const float m2 = __shfl_xor_sync(0xffffffffu, w.m, o);
+      const float s2 = __shfl_xor_sync(0xffffffffu, w.s, o);
+      const float u2 = __shfl_xor_sync(0xffffffffu, w.u, o);
+      w.merge(m2, s2, u2);
+    }
+    if (lane == 0) {
+      total[0] = w.m;
+      total[1] = w.s;
+      total[2] = w.u;
+    }
+    if (a.k > 0) {  // the k-th largest of the 32 maxima (ties by position)
+      const uint32_t mine = gmax[lane];
+      int rank = 0;
+#pragma unroll
+      for (int j = 0; j < 32; ++j) {
+        const uint32_t other = __shfl_sync(0xffffffffu, mine, j);
+        rank += (other > mine || (other == mine && j < lane)) ? 1 : 0;
+      }
+      // a maximum at the floor says nothing about values below it: all are candidates
+      if (rank == a.k - 1) bound_s = mine <= order_key(-kFar) ? 0u : mine;
+    }
+  }
+  __syncthreads();
+  Acc all;
+  all.m = total[0];
+  all.c = all.m == -INFINITY ? 0.0f : all.m * kLog2e;
+  all.s = total[1];
+  all.u = total[2];
+  float row_max = all.m, log_s, entropy;
+  if (all.m > -kFar && all.m < kFar) {
+    const float log2_s = log2f(all.s);
+    log_s = kLn2 * (log2_s - fmaf(all.m, kLog2e, -all.c));
+    entropy = kLn2 * (log2_s - all.u / all.s);
+  } else {  // nothing but masked tokens (or NaN), or values near the type's end: the sums about the row's own maximum
+    float m = -INFINITY;
+    for (int j = tid; j < a.V; j += kThreads) m = fmaxf(m, Elem<T>::one(x + j));
+    row_max = block_max(m, red[0], lane, warp);
+    AccExact ex;
+    ex.m = row_max;
+    for (int j = tid; j < a.V; j += kThreads) {
+      const float v[1] = {Elem<T>::one(x + j)};
+      ex.add(v);
+    }
+    ex.s = block_sum(ex.s, red[1], lane, warp);
+    ex.u = block_sum(ex.u, red[2], lane, warp);
+    log_s = row_max == -INFINITY ? NAN : logf(ex.s);  // nothing above -inf: 0 / 0
+    entropy = log_s - ex.u / ex.s;
+  }
+  all.m = row_max;
   if (tid == 0) {
     a.lp[row] = (Elem<T>::one(x + t) - all.m) - log_s;
-    a.ent[row] = log_s - all.u / all.s;
+    a.ent[row] = entropy;
     a.ms[2 * static_cast<long long>(row)] = all.m;
     a.ms[2 * static_cast<long long>(row) + 1] = log_s;
   }
   if (a.k == 0) return;
-  if (warp == 0) {  // the k-th largest of the 32 maxima (ties by position)
-    const uint32_t mine = gmax[lane];
-    int rank = 0;
-#pragma unroll
-    for (int j = 0; j < 32; ++j) {
-      const uint32_t other = __shfl_sync(0xffffffffu, mine, j);
-      rank += (other > mine || (other == mine && j < lane)) ? 1 : 0;
-    }
-    if (rank == a.k - 1) bound_s = mine;
-  }
-  __syncthreads();
   const uint32_t bound = bound_s;
   auto offer = [&](float v, int idx) {
     if (order_key(v) >= bound) {
@@ -262,8 +369,10 @@ __global__ void __launch_bounds__(kThreads) token_stats_fwd_kernel(const FwdArgs
   };
   if (own_max >= bound) {
     for (int j = tid; j < rs.nvec; j += kThreads) {
+      const uint4 q = rs.body[j];
       float v[kVec];
-      Elem<T>::unpack(rs.body[j], v);
+      if (order_key(Elem<T>::floored(q, v)) < bound) continue;  // most vectors
+      Elem<T>::unpack(q, v);
 #pragma unroll
       for (int e = 0; e < kVec; ++e) offer(v[e], rs.head + j * kVec + e);
     }
