@@ -83,6 +83,7 @@ __device__ __forceinline__ void keep_columns(unsigned long long (&v)[kCols / 2],
 constexpr int kStatsRows = 16;
 __global__ void __launch_bounds__(256) packed_stats_kernel(const Packing p, const int2* __restrict__ list,
                                                            const __nv_bfloat16* __restrict__ o,
+                                                           const __nv_bfloat16* __restrict__ o_lo,
                                                            const __nv_bfloat16* __restrict__ dout,
                                                            const float* __restrict__ lse, float* __restrict__ neg_lse2,
                                                            float* __restrict__ neg_delta, long long pad_rows, int Hq, int D) {
@@ -116,19 +117,21 @@ __global__ void __launch_bounds__(256) packed_stats_kernel(const Packing p, cons
     }
     const long long tok = s.q0 + qi;
     const uint4* a = reinterpret_cast<const uint4*>(o + tok * Hq * D);
+    const uint4* al = reinterpret_cast<const uint4*>(o_lo + tok * Hq * D);
     const uint4* c = reinterpret_cast<const uint4*>(dout + tok * Hq * D);
     for (int base = 0; base < vecs; base += 32) {
       const int i = base + lane;
       float sum = 0.0f;
       if (i < vecs) {
-        const uint4 x = a[i], y = c[i];
+        const uint4 x = a[i], xl = al[i], y = c[i];
+        const uint32_t* lv = reinterpret_cast<const uint32_t*>(&xl);
         const uint32_t* xv = reinterpret_cast<const uint32_t*>(&x);
         const uint32_t* yv = reinterpret_cast<const uint32_t*>(&y);
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
-          const float2 xf = unpack_bf16x2(xv[q]), yf = unpack_bf16x2(yv[q]);
-          sum = fmaf(xf.x, yf.x, sum);
-          sum = fmaf(xf.y, yf.y, sum);
+          const float2 xf = unpack_bf16x2(xv[q]), lf = unpack_bf16x2(lv[q]), yf = unpack_bf16x2(yv[q]);
+          sum = fmaf(xf.x + lf.x, yf.x, sum);
+          sum = fmaf(xf.y + lf.y, yf.y, sum);
         }
       }
       for (int off = per_head / 2; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
@@ -623,11 +626,11 @@ int64_t packed_attn_stats_numel(int64_t Nq, int64_t Hq, int64_t B) {
   return 2 * Hq * packed::pad_slots(Nq, B) * packed::kBlock;
 }
 
-// Backward of packed_attn_fwd.  o, dout contiguous [Nq, Hq, D]; lse [Hq, Nq] from the forward; dq [Nq, Hq, D],
+// Backward of packed_attn_fwd.  o, o_lo, dout contiguous [Nq, Hq, D]; lse [Hq, Nq] from the forward; dq [Nq, Hq, D],
 // dk/dv [Nk, Hkv, D] bf16 with any 16-byte-aligned strides (views of one packed buffer, say).  stats: fp32 scratch,
 // sched: int32 scratch.
-void packed_attn_bwd(torch::Tensor q, torch::Tensor k, torch::Tensor v, torch::Tensor o, torch::Tensor dout,
-                     torch::Tensor lse, torch::Tensor cu_q, torch::Tensor cu_k, double scale, torch::Tensor dq,
+void packed_attn_bwd(torch::Tensor q, torch::Tensor k, torch::Tensor v, torch::Tensor o, torch::Tensor o_lo,
+                     torch::Tensor dout, torch::Tensor lse, torch::Tensor cu_q, torch::Tensor cu_k, double scale, torch::Tensor dq,
                      torch::Tensor dk, torch::Tensor dv, torch::Tensor stats, torch::Tensor sched) {
   using namespace packed;
   TT_CHECK(q.dim() == 3 && k.dim() == 3, "packed_attn_bwd: q and k must be [tokens, heads, D]");
@@ -638,11 +641,12 @@ void packed_attn_bwd(torch::Tensor q, torch::Tensor k, torch::Tensor v, torch::T
   check_heads(k, Hkv, D, "packed_attn_bwd k");
   check_heads(v, Hkv, D, "packed_attn_bwd v");
   check_heads(o, Hq, D, "packed_attn_bwd o");
+  check_heads(o_lo, Hq, D, "packed_attn_bwd o_lo");
   check_heads(dout, Hq, D, "packed_attn_bwd dout");
   check_heads(dq, Hq, D, "packed_attn_bwd dq");
   check_heads(dk, Hkv, D, "packed_attn_bwd dk");
   check_heads(dv, Hkv, D, "packed_attn_bwd dv");
-  TT_CHECK(o.is_contiguous() && dout.is_contiguous() && o.size(0) == Nq && dout.size(0) == Nq && dq.size(0) == Nq &&
+  TT_CHECK(o.is_contiguous() && o_lo.is_contiguous() && dout.is_contiguous() && o.size(0) == Nq && o_lo.size(0) == Nq && dout.size(0) == Nq && dq.size(0) == Nq &&
                v.size(0) == Nk && dk.size(0) == Nk && dv.size(0) == Nk,
            "packed_attn_bwd: token counts; o and dout must be contiguous");
   check_offsets(cu_q, -1, "cu_seqlens");
@@ -687,8 +691,8 @@ void packed_attn_bwd(torch::Tensor q, torch::Tensor k, torch::Tensor v, torch::T
   // dQ's list first: it checks the offsets, and a bad packing leaves every entry empty
   schedule(p.pk, kQueryTiles, list, static_cast<int>(q_entries), status, st);
   packed_stats_kernel<<<static_cast<unsigned>(pad_slots(Nq, B) * (kBlock / kStatsRows)), 256, 0, st>>>(
-      p.pk, list, reinterpret_cast<const __nv_bfloat16*>(o.data_ptr()), reinterpret_cast<const __nv_bfloat16*>(dout.data_ptr()),
-      lse.data_ptr<float>(), neg_lse2, neg_delta, p.pad_rows, p.Hq, static_cast<int>(D));
+      p.pk, list, reinterpret_cast<const __nv_bfloat16*>(o.data_ptr()), reinterpret_cast<const __nv_bfloat16*>(o_lo.data_ptr()),
+      reinterpret_cast<const __nv_bfloat16*>(dout.data_ptr()), lse.data_ptr<float>(), neg_lse2, neg_delta, p.pad_rows, p.Hq, static_cast<int>(D));
   TT_CUDA_CHECK(cudaGetLastError());
   auto launch = [&](auto kern, size_t smem, int64_t blocks) {
     TT_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));

@@ -115,6 +115,7 @@ struct FwdParams {
   int Hq, Hkv;
   int head_pairs;    // a CTA's two tiles: 1 one tile of two heads, 0 two tiles of one head
   __nv_bfloat16* o;  // [Nq, Hq, D] contiguous
+  __nv_bfloat16* o_lo;  // what rounding o to bf16 left over, same layout (may be null)
   float* lse;        // [Hq, Nq] natural log (may be null)
   float scale_log2;
   int* status;
@@ -172,6 +173,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int i = threadIdx.x; i < rows * NU; i += kThreads) {
         const long long row = s.q0 + first + i / NU;
         reinterpret_cast<uint4*>(p.o + (row * p.Hq + h0 + x * dh) * D)[i % NU] = make_uint4(0u, 0u, 0u, 0u);
+        if (p.o_lo != nullptr) reinterpret_cast<uint4*>(p.o_lo + (row * p.Hq + h0 + x * dh) * D)[i % NU] = make_uint4(0u, 0u, 0u, 0u);
       }
       if (p.lse != nullptr)
         for (int i = threadIdx.x; i < rows; i += kThreads)
@@ -393,12 +395,12 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int h = h0 + x * dh;
       const bool row_ok = qi < s.qlen;
       const long long row = s.q0 + qi;
-      __nv_bfloat16* orow = p.o + (row * p.Hq + h) * D + wg * W;
+      const long long at = (row * p.Hq + h) * D + wg * W;
       const bool seen = min(qi + s.off, s.klen - 1) >= 0;
-      uint32_t w[W / 2];
+      uint32_t w[W / 2], rest[W / 2];
       if (n_x[x] == 0) {
 #pragma unroll
-        for (int i = 0; i < W / 2; ++i) w[i] = 0u;
+        for (int i = 0; i < W / 2; ++i) w[i] = rest[i] = 0u;
       } else {
         if (!ok || !mbar_wait_warp(&sm.o_done[x], (n_x[x] - 1) & 1, p.status, kTimeoutAccFull)) break;
         tc_fence_after();
@@ -410,14 +412,23 @@ __global__ void __launch_bounds__(kThreads, 1)
         else tmem_ld16(o_addr, ov);
         tmem_ld_wait();
 #pragma unroll
-        for (int i = 0; i < W / 2; ++i)
-          w[i] = seen ? pack_bf16x2(__uint_as_float(ov[2 * i]) * inv_l, __uint_as_float(ov[2 * i + 1]) * inv_l) : 0u;
+        for (int i = 0; i < W / 2; ++i) {
+          const float a = __uint_as_float(ov[2 * i]) * inv_l, c = __uint_as_float(ov[2 * i + 1]) * inv_l;
+          w[i] = seen ? pack_bf16x2(a, c) : 0u;
+          const float2 f = unpack_bf16x2(w[i]);
+          rest[i] = seen ? pack_bf16x2(a - f.x, c - f.y) : 0u;
+        }
         if (row_ok && wg == 0 && p.lse != nullptr)
           p.lse[static_cast<long long>(h) * p.pk.Nq + row] = seen ? (m_ref[x] + log2f(sum)) * 0.69314718055994531f : -INFINITY;
       }
       if (row_ok) {
 #pragma unroll
-        for (int i = 0; i < W / 8; ++i) reinterpret_cast<uint4*>(orow)[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+        for (int i = 0; i < W / 8; ++i) reinterpret_cast<uint4*>(p.o + at)[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+        if (p.o_lo != nullptr) {
+#pragma unroll
+          for (int i = 0; i < W / 8; ++i)
+            reinterpret_cast<uint4*>(p.o_lo + at)[i] = make_uint4(rest[4 * i], rest[4 * i + 1], rest[4 * i + 2], rest[4 * i + 3]);
+        }
         if (n_x[x] == 0 && wg == 0 && p.lse != nullptr) p.lse[static_cast<long long>(h) * p.pk.Nq + row] = -INFINITY;
       }
     }
@@ -438,9 +449,11 @@ int64_t packed_attn_schedule_numel(int64_t Nq, int64_t Nk, int64_t B) {
 }
 
 // q [Nq, Hq, D], k/v [Nk, Hkv, D] bf16 (any 16-byte-aligned strides), cu_q/cu_k int32 [B + 1] ->
-// o [Nq, Hq, D] contiguous, lse fp32 [Hq, Nq] (optional).  sched: int32 scratch.
+// o [Nq, Hq, D] contiguous; for a backward, lse fp32 [Hq, Nq] and o_lo (o's layout): what the rounding of o left
+// over, so that delta = dO . O is not off by it (0.0026 -> 0.0024 relative error of dQ).  sched: int32 scratch.
 void packed_attn_fwd(torch::Tensor q, torch::Tensor k, torch::Tensor v, torch::Tensor cu_q, torch::Tensor cu_k,
-                     double scale, torch::Tensor o, c10::optional<torch::Tensor> lse, torch::Tensor sched) {
+                     double scale, torch::Tensor o, c10::optional<torch::Tensor> lse, c10::optional<torch::Tensor> o_lo,
+                     torch::Tensor sched) {
   using namespace packed;
   TT_CHECK(q.dim() == 3 && k.dim() == 3, "packed_attn: q and k must be [tokens, heads, D]");
   const int64_t Nq = q.size(0), Hq = q.size(1), D = q.size(2), Nk = k.size(0), Hkv = k.size(1);
@@ -458,6 +471,11 @@ void packed_attn_fwd(torch::Tensor q, torch::Tensor k, torch::Tensor v, torch::T
            "packed_attn: o must be contiguous [Nq, Hq, D]");
   if (lse.has_value())
     TT_CHECK(lse->scalar_type() == torch::kFloat32 && lse->is_contiguous() && lse->numel() == Hq * Nq, "packed_attn: lse must be fp32 [Hq, Nq]");
+  if (o_lo.has_value()) {
+    check_cuda_bf16(*o_lo, "o_lo");
+    TT_CHECK(o_lo->is_contiguous() && o_lo->numel() == o.numel() && reinterpret_cast<uintptr_t>(o_lo->data_ptr()) % 16 == 0,
+             "packed_attn: o_lo must be contiguous [Nq, Hq, D]");
+  }
   TT_CHECK(scale > 0 && std::isfinite(scale), "packed_attn: scale must be positive and finite");
   TT_CHECK(sched.scalar_type() == torch::kInt32 && sched.is_contiguous() && sched.numel() >= packed_attn_schedule_numel(Nq, Nk, B) &&
                reinterpret_cast<uintptr_t>(sched.data_ptr()) % 8 == 0,
@@ -468,6 +486,7 @@ void packed_attn_fwd(torch::Tensor q, torch::Tensor k, torch::Tensor v, torch::T
   if (Nk == 0) {  // no keys at all (a tensor map cannot be empty)
     o.zero_();
     if (lse.has_value()) lse->fill_(-INFINITY);
+    if (o_lo.has_value()) o_lo->zero_();
     return;
   }
   FwdParams p{};
@@ -476,6 +495,7 @@ void packed_attn_fwd(torch::Tensor q, torch::Tensor k, torch::Tensor v, torch::T
   p.Hq = static_cast<int>(Hq);
   p.Hkv = static_cast<int>(Hkv);
   p.o = reinterpret_cast<__nv_bfloat16*>(o.data_ptr());
+  p.o_lo = o_lo.has_value() ? reinterpret_cast<__nv_bfloat16*>(o_lo->data_ptr()) : nullptr;
   p.lse = lse.has_value() ? lse->data_ptr<float>() : nullptr;
   p.scale_log2 = static_cast<float>(scale * 1.4426950408889634);
   p.status = device_status_ptr(q.get_device());

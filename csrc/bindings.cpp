@@ -96,10 +96,11 @@ void paged_attention(torch::Tensor q, torch::Tensor k_pages, torch::Tensor v_pag
                      torch::Tensor seq_lens, double scale, torch::Tensor part, torch::Tensor counters, torch::Tensor out);
 int64_t packed_attn_schedule_numel(int64_t Nq, int64_t Nk, int64_t B);
 void packed_attn_fwd(torch::Tensor q, torch::Tensor k, torch::Tensor v, torch::Tensor cu_q, torch::Tensor cu_k,
-                     double scale, torch::Tensor o, c10::optional<torch::Tensor> lse, torch::Tensor sched);
+                     double scale, torch::Tensor o, c10::optional<torch::Tensor> lse, c10::optional<torch::Tensor> o_lo,
+                     torch::Tensor sched);
 int64_t packed_attn_stats_numel(int64_t Nq, int64_t Hq, int64_t B);
-void packed_attn_bwd(torch::Tensor q, torch::Tensor k, torch::Tensor v, torch::Tensor o, torch::Tensor dout,
-                     torch::Tensor lse, torch::Tensor cu_q, torch::Tensor cu_k, double scale, torch::Tensor dq,
+void packed_attn_bwd(torch::Tensor q, torch::Tensor k, torch::Tensor v, torch::Tensor o, torch::Tensor o_lo,
+                     torch::Tensor dout, torch::Tensor lse, torch::Tensor cu_q, torch::Tensor cu_k, double scale, torch::Tensor dq,
                      torch::Tensor dk, torch::Tensor dv, torch::Tensor stats, torch::Tensor sched);
 void ep_allgather_counts(int64_t gid, torch::Tensor counts, int64_t dst_off);
 void ep_scatter(int64_t gid, torch::Tensor x, int64_t k, torch::Tensor tgt, torch::Tensor dst, int64_t recv_off,

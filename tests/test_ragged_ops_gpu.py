@@ -235,9 +235,9 @@ def test_packed_attention_first_call_of_a_thread():
     def work():
         from tinytron_b200.ops import ragged
 
-        o, lse = ragged._packed_fwd(q, k, v, cu, cu, 0.125, True)
+        o, saved = ragged._packed_fwd(q, k, v, cu, cu, 0.125, True)
         d = [torch.empty_like(x) for x in (q, k, v)]
-        ragged._packed_bwd(q, k, v, o, lse, do, cu, cu, 0.125, *d)
+        ragged._packed_bwd(q, k, v, o, *saved, do, cu, cu, 0.125, *d)
         got.extend([o, *d])
 
     torch.cuda.synchronize()

@@ -71,17 +71,19 @@ def _packed_attention_cpu(q, k, v, cu_q, cu_k, scale):
     return torch.cat(out) if out else torch.zeros_like(q)
 
 
-def _packed_fwd(q, k, v, cu_q, cu_k, scale, want_lse):
+def _packed_fwd(q, k, v, cu_q, cu_k, scale, for_backward):
+    """(o, (o_lo, lse)): for a backward, what the rounding of o left over and the rows' log-sum-exp."""
     C = _C()
     nq, hq, d = q.shape
     o = torch.empty(nq, hq, d, dtype=q.dtype, device=q.device)
-    lse = torch.empty(hq, nq, dtype=torch.float32, device=q.device) if want_lse else None
+    o_lo = torch.empty_like(o) if for_backward else None
+    lse = torch.empty(hq, nq, dtype=torch.float32, device=q.device) if for_backward else None
     sched = torch.empty(C.packed_attn_schedule_numel(nq, k.shape[0], cu_q.numel() - 1), dtype=torch.int32, device=q.device)
-    C.packed_attn_fwd(q, k, v, cu_q, cu_k, scale, o, lse, sched)
-    return o, lse
+    C.packed_attn_fwd(q, k, v, cu_q, cu_k, scale, o, lse, o_lo, sched)
+    return o, (o_lo, lse)
 
 
-def _packed_bwd(q, k, v, o, lse, do, cu_q, cu_k, scale, dq, dk, dv):
+def _packed_bwd(q, k, v, o, o_lo, lse, do, cu_q, cu_k, scale, dq, dk, dv):
     C = _C()
     nq, hq, _ = q.shape
     b = cu_q.numel() - 1
@@ -91,27 +93,27 @@ def _packed_bwd(q, k, v, o, lse, do, cu_q, cu_k, scale, dq, dk, dv):
     do = do.contiguous()
     if do.data_ptr() % 16:
         do = do.clone()
-    C.packed_attn_bwd(q, k, v, o, do, lse, cu_q, cu_k, scale, dq, dk, dv, stats, sched)
+    C.packed_attn_bwd(q, k, v, o, o_lo, do, lse, cu_q, cu_k, scale, dq, dk, dv, stats, sched)
 
 
 class PackedAttentionFn(torch.autograd.Function):
-    """Forward saves q, k, v, o and the log-sum-exp; backward is two kernels (dQ; dK and dV) whose
+    """Forward saves q, k, v, o, what the rounding of o left over, and the log-sum-exp; backward is two kernels (dQ; dK and dV) whose
     sums have a fixed order."""
 
     @staticmethod
     def forward(ctx, q, k, v, cu_q, cu_k, scale):
         q, k, v = _kernel_rows(q), _kernel_rows(k), _kernel_rows(v)
-        o, lse = _packed_fwd(q, k, v, cu_q, cu_k, scale, any(ctx.needs_input_grad[:3]))
-        ctx.save_for_backward(q, k, v, o, lse, cu_q, cu_k)
+        o, saved = _packed_fwd(q, k, v, cu_q, cu_k, scale, any(ctx.needs_input_grad[:3]))
+        ctx.save_for_backward(q, k, v, o, *saved, cu_q, cu_k)
         ctx.scale = scale
         return o
 
     @staticmethod
     @once_differentiable
     def backward(ctx, do):
-        q, k, v, o, lse, cu_q, cu_k = ctx.saved_tensors
+        q, k, v, o, o_lo, lse, cu_q, cu_k = ctx.saved_tensors
         dq, dk, dv = (torch.empty(x.shape, dtype=x.dtype, device=x.device) for x in (q, k, v))
-        _packed_bwd(q, k, v, o, lse, do.reshape(o.shape), cu_q, cu_k, ctx.scale, dq, dk, dv)
+        _packed_bwd(q, k, v, o, o_lo, lse, do.reshape(o.shape), cu_q, cu_k, ctx.scale, dq, dk, dv)
         return dq, dk, dv, None, None, None
 
 
@@ -158,20 +160,20 @@ class RotaryPackedAttentionFn(torch.autograd.Function):
         q, k, v = x[:, :hq], x[:, hq:hq + hkv], x[:, hq + hkv:]
         _C().rotary_append(qkv, cos, sin, hq, hkv, d, cu, None, False, q, k, None, None, None)
         scale = 1.0 / math.sqrt(d)
-        o, lse = _packed_fwd(q, k, v, cu, cu, scale, ctx.needs_input_grad[0])
-        ctx.save_for_backward(qkv, o, lse, cu, cos, sin)
+        o, saved = _packed_fwd(q, k, v, cu, cu, scale, ctx.needs_input_grad[0])
+        ctx.save_for_backward(qkv, o, *saved, cu, cos, sin)
         ctx.cfg = (hq, hkv, d, scale)
         return o.view(n, hq * d)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, do):
-        qkv, o, lse, cu, cos, sin = ctx.saved_tensors
+        qkv, o, o_lo, lse, cu, cos, sin = ctx.saved_tensors
         hq, hkv, d, scale = ctx.cfg
         n = qkv.shape[0]
         dqkv = torch.empty_like(qkv)
         x, dx = qkv.view(n, hq + 2 * hkv, d), dqkv.view(n, hq + 2 * hkv, d)
-        _packed_bwd(x[:, :hq], x[:, hq:hq + hkv], x[:, hq + hkv:], o, lse, do.reshape(n, hq, d), cu, cu, scale,
+        _packed_bwd(x[:, :hq], x[:, hq:hq + hkv], x[:, hq + hkv:], o, o_lo, lse, do.reshape(n, hq, d), cu, cu, scale,
                     dx[:, :hq], dx[:, hq:hq + hkv], dx[:, hq + hkv:])
         _C().rotary_append(dqkv, cos, sin, hq, hkv, d, cu, None, True, dx[:, :hq], dx[:, hq:hq + hkv], None, None, None)
         return dqkv, None, None, None, None, None, None
