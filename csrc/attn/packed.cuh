@@ -182,6 +182,15 @@ inline Packing packing_of(const torch::Tensor& q, const torch::Tensor& k, const 
   return p;
 }
 
+// Allows a kernel `smem` bytes of shared memory, once per device (its size is the kernel's own constant).
+template <auto kKernel>
+inline void allow_smem(size_t smem, int device) {
+  static std::once_flag once[64];
+  std::call_once(once[device & 63], [&] {
+    TT_CUDA_CHECK(cudaFuncSetAttribute(kKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
+  });
+}
+
 enum ScheduleKind { kQueryPairs = 0, kQueryTiles = 1, kKeyTiles = 2 };
 
 // List (int2 {sequence, tile}, longest first, {-1, 0} past the end) of a packing's query tile pairs, query

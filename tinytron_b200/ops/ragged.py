@@ -145,6 +145,8 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
         return _packed_attention_cpu(q, k, v, cu_q, cu_k, scale)
     if q.dtype != torch.bfloat16 or q.shape[2] not in (64, 128):
         raise ValueError(f"packed_attention runs bf16 with head_dim 64 or 128 on CUDA, got {q.dtype} and {q.shape[2]}")
+    if not (torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad)):
+        return _packed_fwd(_kernel_rows(q), _kernel_rows(k), _kernel_rows(v), cu_q, cu_k, scale, False)[0]
     return PackedAttentionFn.apply(q, k, v, cu_q, cu_k, scale)
 
 
@@ -409,16 +411,21 @@ class TokenStats(NamedTuple):
     top_ids: torch.Tensor
 
 
+def _token_stats_fwd(logits, targets, top_k, ignore_index):
+    n = logits.shape[0]
+    f = dict(dtype=torch.float32, device=logits.device)
+    lp, ent, ms, top = torch.empty(n, **f), torch.empty(n, **f), torch.empty(n, 2, **f), torch.empty(n, top_k, **f)
+    ids = torch.empty(n, top_k, dtype=torch.long, device=logits.device)
+    _C().token_stats_fwd(logits, targets, top_k, ignore_index, lp, ent, ms, top, ids)
+    return lp, ent, top, ids, ms
+
+
 class TokenStatsFn(torch.autograd.Function):
     """One pass over the logits forward, one read and one write backward (csrc/fused/token_stats.cu)."""
 
     @staticmethod
     def forward(ctx, logits, targets, top_k, ignore_index):
-        n = logits.shape[0]
-        f = dict(dtype=torch.float32, device=logits.device)
-        lp, ent, ms, top = torch.empty(n, **f), torch.empty(n, **f), torch.empty(n, 2, **f), torch.empty(n, top_k, **f)
-        ids = torch.empty(n, top_k, dtype=torch.long, device=logits.device)
-        _C().token_stats_fwd(logits, targets, top_k, ignore_index, lp, ent, ms, top, ids)
+        lp, ent, top, ids, ms = _token_stats_fwd(logits, targets, top_k, ignore_index)
         ctx.save_for_backward(logits, targets, ent, ms, ids)
         ctx.cfg = (top_k, ignore_index)
         ctx.set_materialize_grads(False)
@@ -473,7 +480,10 @@ def token_stats(logits: torch.Tensor, targets: torch.Tensor, top_k: int = 0, ign
     if logits.is_cuda:
         if v and x.stride(-1) != 1:
             x = x.contiguous()
-        lp, ent, top, ids = TokenStatsFn.apply(x, t, top_k, ignore_index)
+        if torch.is_grad_enabled() and x.requires_grad:
+            lp, ent, top, ids = TokenStatsFn.apply(x, t, top_k, ignore_index)
+        else:
+            lp, ent, top, ids, _ = _token_stats_fwd(x, t, top_k, ignore_index)
     else:
         lp, ent, top, ids = _token_stats_cpu(x, t, top_k, ignore_index)
     return TokenStats(lp.view(lead), ent.view(lead), top.view(*lead, top_k), ids.view(*lead, top_k))
