@@ -40,15 +40,10 @@ constexpr uint32_t kComputeThreads = kGroups * 128;
 constexpr int kRegIssue = 64, kRegCompute = 104;
 static_assert(kRegIssue + kGroups * kRegCompute <= (1 + kGroups) * 96, "register split exceeds the launch");
 
-__device__ __forceinline__ unsigned long long f2_mul(unsigned long long a, unsigned long long b) {
-  unsigned long long d;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-  return d;
-}
-
 // Probabilities of 32 scores in pairs: 2^(s scale_log2 + add), add = -lse2 of the column (or row); kPoly of eight
-// exponentials on the FMA pipe instead of MUFU.
-template <int kPoly, typename Add>
+// exponentials on the FMA pipe instead of MUFU.  kAny: a NaN addend (a row that saw a NaN or an infinite score) gives NaN
+// in every column; dQ's kernel need not, its dS is NaN by delta.
+template <int kPoly, bool kAny, typename Add>
 __device__ __forceinline__ void probabilities(const uint32_t (&raw)[kCols], unsigned long long (&pv)[kCols / 2],
                                               float scale_log2, Add add) {
   const unsigned long long s2 = f2_pack(scale_log2, scale_log2);
@@ -57,10 +52,11 @@ __device__ __forceinline__ void probabilities(const uint32_t (&raw)[kCols], unsi
     float a, b;
     f2_unpack(f2_fma(f2_pack(__uint_as_float(raw[2 * i]), __uint_as_float(raw[2 * i + 1])), s2, add(i)), a, b);
     if ((i & 3) == 3) {
-      exp2_poly2(a, b);
+      if (kAny) exp2_poly2_any(a, b);
+      else exp2_poly2(a, b);
     } else {
       a = ex2_mufu(a);
-      b = (kPoly == 3 && (i & 3) == 1) ? exp2_poly(b) : ex2_mufu(b);
+      b = (kPoly == 3 && (i & 3) == 1) ? (kAny ? exp2_poly_any(b) : exp2_poly(b)) : ex2_mufu(b);
     }
     pv[i] = f2_pack(a, b);
   }
@@ -341,7 +337,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       tmem_ld32(s_addr, raw);
       const ulonglong2* nl = reinterpret_cast<const ulonglong2*>(sm.neg_lse2[buf] + wg * kCols);
       tmem_ld_wait();
-      probabilities<3>(raw, pv, p.scale_log2, [&](int i) { return (i & 1) ? nl[i >> 1].y : nl[i >> 1].x; });
+      probabilities<3, true>(raw, pv, p.scale_log2, [&](int i) { return (i & 1) ? nl[i >> 1].y : nl[i >> 1].x; });
       const int lo = key_row - qt * kBlock, hi = end_row - qt * kBlock;
       if (lo > 0 || hi < kCols) keep_columns(pv, lo, hi);
       uint32_t pk[16];
@@ -582,7 +578,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         uint32_t raw[kCols];
         tmem_ld32(s_addr, raw);
         tmem_ld_wait();
-        probabilities<2>(raw, pv, p.scale_log2, [&](int) { return nl2; });
+        probabilities<2, false>(raw, pv, p.scale_log2, [&](int) { return nl2; });
       }
       if (!mbar_wait_warp(&sm.dp_full, j & 1, p.status, kTimeoutAccFull)) {
         ok = false;

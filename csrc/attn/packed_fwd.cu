@@ -15,6 +15,9 @@
 // tile's softmax is on the critical path between its products.  A last, partial key tile takes rows of the next sequence:
 // their probabilities are zero, but zero times an infinity or NaN of a neighbour would not be, so
 // the softmax warps clear those rows of V before the product.
+// Scores that are not finite stay what they are: -inf and masked keys weigh exactly zero, a NaN or +inf makes the rows that
+// see it NaN (exp2_poly_any), as the definition does.  A NaN or infinity in V reaches the rows that see it, and may
+// reach rows of the same sequence in the same tile that do not (zero times it).
 //
 // Bound by the softmax between a tile's two products (TMEM read, maxima, exponentials, P back), which the other
 // tile's products hide only in part.  14 sequences, 16384 tokens, 16/4 heads, d 128 (132 GFLOP of visible
@@ -350,10 +353,10 @@ __global__ void __launch_bounds__(kThreads, 1)
           f2_unpack(f2_fma(f2_pack(__uint_as_float(raw[i]), __uint_as_float(raw[i + 1])), s2, nm2), e0, e1);
           // part of the exponentials on the FMA pipe, so that MUFU does not bound the tile
           if ((i & 7) == 6 || (kPolyEighths == 4 && (i & 7) == 2)) {
-            exp2_poly2(e0, e1);
+            exp2_poly2_any(e0, e1);
           } else {
             e0 = ex2_mufu(e0);
-            e1 = (kPolyEighths == 3 && (i & 7) == 2) ? exp2_poly(e1) : ex2_mufu(e1);
+            e1 = (kPolyEighths == 3 && (i & 7) == 2) ? exp2_poly_any(e1) : ex2_mufu(e1);
           }
           if (i & 2) sb = f2_add(sb, f2_pack(e0, e1));
           else sa = f2_add(sa, f2_pack(e0, e1));
