@@ -442,6 +442,15 @@ class TokenStatsFn(torch.autograd.Function):
         return grad, None, None, None
 
 
+def _ranking(x):
+    """Columns of each row by falling logit, equal ones by their index, NaN last.  Not by log-prob: distinct logits
+    may round to one."""
+    nan = x.isnan()
+    order = torch.sort(x.masked_fill(nan, -math.inf), dim=-1, descending=True, stable=True).indices
+    last = torch.sort(nan.gather(1, order).to(torch.uint8), dim=-1, stable=True).indices  # NaN behind -inf too
+    return order.gather(1, last)
+
+
 def _token_stats_cpu(logits, targets, top_k, ignore_index):
     scored = targets != ignore_index
     t = targets.clamp(min=0)
@@ -453,7 +462,7 @@ def _token_stats_cpu(logits, targets, top_k, ignore_index):
     lp = torch.where(scored, y.gather(1, t[:, None])[:, 0], zero)
     p = y.exp()
     ent = torch.where(scored, -(p * torch.where(p > 0, y, zero)).sum(-1), zero)  # p log p is 0 where p is
-    ids = torch.sort(y.detach(), dim=-1, descending=True, stable=True).indices[:, :top_k]
+    ids = _ranking(logits.detach())[:, :top_k]
     top = torch.where(scored[:, None], y.gather(1, ids), zero)
     return lp, ent, top, torch.where(scored[:, None], ids, torch.full_like(ids, -1))
 
