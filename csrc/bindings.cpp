@@ -78,10 +78,10 @@ void decode_advance(torch::Tensor nxt, torch::Tensor tokens, int64_t P, torch::T
 void decode_attention(torch::Tensor q, torch::Tensor k_pages, torch::Tensor v_pages, torch::Tensor page_table,
                       c10::optional<torch::Tensor> len_dev, int64_t len_host, int64_t splits, double scale,
                       torch::Tensor o_part, torch::Tensor ml_part, torch::Tensor out);
-void token_stats_fwd(torch::Tensor logits, torch::Tensor targets, int64_t k, int64_t ignore_index, torch::Tensor lp,
-                     torch::Tensor ent, torch::Tensor ms, torch::Tensor top_lp, torch::Tensor top_id);
-void token_stats_bwd(torch::Tensor logits, torch::Tensor targets, int64_t k, int64_t ignore_index, torch::Tensor ent,
-                     torch::Tensor ms, torch::Tensor top_id, c10::optional<torch::Tensor> g_lp,
+void token_stats_fwd(torch::Tensor logits, torch::Tensor targets, int64_t k, int64_t ignore_index, double temperature,
+                     torch::Tensor lp, torch::Tensor ent, torch::Tensor ms, torch::Tensor top_lp, torch::Tensor top_id);
+void token_stats_bwd(torch::Tensor logits, torch::Tensor targets, int64_t k, int64_t ignore_index, double temperature,
+                     torch::Tensor ent, torch::Tensor ms, torch::Tensor top_id, c10::optional<torch::Tensor> g_lp,
                      c10::optional<torch::Tensor> g_ent, c10::optional<torch::Tensor> g_top, torch::Tensor grad);
 void rotary_append(torch::Tensor qkv, torch::Tensor cos_t, torch::Tensor sin_t, int64_t Hq, int64_t Hkv, int64_t D,
                    torch::Tensor cu, c10::optional<torch::Tensor> start, bool inverse, torch::Tensor q_out,

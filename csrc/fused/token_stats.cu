@@ -1,20 +1,22 @@
 // Statistics of given tokens under rows of logits, and their gradient.
 //
-// For a row x [V] with target t and k alternatives (m = max x, d_j = x_j - m, s = sum e^d_j,
-// u = sum e^d_j d_j, p = softmax(x)):
+// For a row x [V] with target t, temperature T and k alternatives (m = max x, d_j = (x_j - m) / T, s = sum e^d_j,
+// u = sum e^d_j d_j, p = softmax(x / T)):
 //   log p(t)  = d_t - log s
 //   entropy   = -sum p log p = log s - u / s
 //   top i     = the i-th largest x (ties: lowest index first), log p = d - log s
-//   d/dx_j    = g_lp (1[j = t] - p_j) - g_ent p_j (log p_j + H) + sum_i g_i (1[j = id_i] - p_j)
+//   T d/dx_j  = g_lp (1[j = t] - p_j) - g_ent p_j (log p_j + H) + sum_i g_i (1[j = id_i] - p_j)
+// 1 / T is applied in fp32 to the logits as they are read, as the sampler does: dividing bf16 logits first would round
+// them a second time, which at T 0.7 moves a log-prob by 0.009 on average.
 // (m, log s) are kept apart for the backward: their sum would round away bits of log s at large m.
 //
-// Forward: one pass, in the log2 domain about c = fl(m log2e).  One FMA forms y_j = x_j log2e - c, so
-// s' = sum 2^y and u' = sum 2^y y share one offset delta = m log2e - c (known exactly from another FMA):
+// Forward: one pass, in the log2 domain about c = fl(m k), k = log2e / T.  One FMA forms y_j = x_j k - c, so
+// s' = sum 2^y and u' = sum 2^y y share one offset delta = m k - c (known exactly from another FMA):
 // entropy = ln2 (log2 s' - u' / s') does not depend on it, log s = ln2 (log2 s' - delta).  An element
 // costs an FMA, an exponential, an add and an FMA; with about 8 cycles a warp the exponential (MUFU) is
 // the most of it, 16 elements a cycle and SM, against 11.6 that memory delivers.  A thread keeps (m, s', u')
 // of its elements and raises m only when a 16-byte vector holds a larger value.  Values below -1e6 (masked
-// tokens) count as -1e6 there; a row with nothing above that is done again exactly.  The alternatives ride along without a second pass over
+// tokens) count as -1e6 there; a row with nothing above that, or of a temperature far from 1, is done again exactly.  The alternatives ride along without a second pass over
 // the row: the k-th largest of the 32 half-warp maxima bounds the k-th largest element from
 // below, so only threads whose own maximum reaches that bound look at their elements again
 // (about k of them), and the few candidates are ranked in shared memory.
@@ -25,6 +27,8 @@
 #include "common/host_utils.h"
 #include "common/ptx.cuh"
 #include "common/fast_exp2.cuh"
+
+#include <cmath>
 
 namespace tt {
 namespace stats {
@@ -115,9 +119,15 @@ __device__ __forceinline__ float max_nan(float a, float b) {  // NaN if either i
 
 constexpr float kFloor = -1e6f;  // what lower values count as in the first pass
 constexpr float kFar = 9e5f;     // a row whose maximum is further from zero is summed again exactly (c would round too much)
+// Temperatures of the one-pass sums.  Up to T = 100 a floored value (1e5 below a maximum above -kFar) is still e^-1000; down
+// to T = 0.001 the c of a thread of masked tokens only (1e6 k) is rounded by at most 64, so its 2^y stay finite and the factor
+// that drops them is a zero times a number.
+constexpr float kMinInvT = 0.01f, kMaxInvT = 1000.0f;
 
 struct Acc {
+  float k = kLog2e;  // log2e / T
   float m = -INFINITY, c = 0.0f, s = 0.0f, u = 0.0f;
+  __device__ __forceinline__ explicit Acc(float k_) : k(k_) {}
   // Moves the sums from reference `from` to a larger one.
   __device__ __forceinline__ void shift(float from, float to) {
     const float dc = from - to;
@@ -126,7 +136,7 @@ struct Acc {
     s *= f;                                     // a NaN of s stays
   }
   __device__ __forceinline__ void raise(float m2) {  // m2 > m
-    const float c2 = m2 * kLog2e;
+    const float c2 = m2 * k;
     if (m != -INFINITY) shift(c, c2);
     m = m2;
     c = c2;
@@ -135,14 +145,14 @@ struct Acc {
   __device__ __forceinline__ void add(const float (&v)[N]) {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const float y = fmaf(v[i], kLog2e, -c);
+      const float y = fmaf(v[i], k, -c);
       const float e = ex2_mufu(y);
       s += e;
       u = fmaf(e, y, u);
     }
   }
   __device__ __forceinline__ void merge(float m2, float s2, float u2) {
-    float c2 = m2 == -INFINITY ? 0.0f : m2 * kLog2e;
+    float c2 = m2 == -INFINITY ? 0.0f : m2 * k;
     if (m2 > m) {
       const float a = m, d = c, x = s, y = u;
       m = m2, c = c2, s = s2, u = u2;
@@ -161,13 +171,13 @@ struct Acc {
 
 // The same sums in natural units about a known maximum, for rows of only masked tokens.
 struct AccExact {
-  float m = -INFINITY, s = 0.0f, u = 0.0f;
+  float inv_t = 1.0f, m = -INFINITY, s = 0.0f, u = 0.0f;
   template <int N>
   __device__ __forceinline__ void add(const float (&v)[N]) {
     const float mm = m == -INFINITY ? 0.0f : m;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const float d = max_nan(v[i] - mm, -1e30f);
+      const float d = max_nan((v[i] - mm) * inv_t, -1e30f);
       const float e = ex2_mufu(d * kLog2e);
       s += e;
       u = fmaf(e, d, u);
@@ -202,6 +212,7 @@ struct FwdArgs {
   const int64_t* targets;
   int64_t ignore;
   int N, V, k;
+  float inv_t;
   float* lp;
   float* ent;
   float* ms;        // [N, 2]: m, log s
@@ -258,7 +269,8 @@ __global__ void __launch_bounds__(kThreads) token_stats_fwd_kernel(const FwdArgs
   const RowSplit<T> rs(x, a.V);
   const int tail = rs.head + rs.nvec * kVec;
   if (tid == 0) n_cand = 0;
-  Acc acc;
+  const float kt = kLog2e * a.inv_t;
+  Acc acc(kt);
   auto take = [&](const uint4& q) {
     float v[kVec];
     const float vm = Elem<T>::floored(q, v);
@@ -303,7 +315,7 @@ __global__ void __launch_bounds__(kThreads) token_stats_fwd_kernel(const FwdArgs
   }
   __syncthreads();
   if (warp == 0) {  // the warps' sums, in the order of a fixed tree
-    Acc w;
+    Acc w(kt);
     if (lane < kThreads / 32) w.merge(red[0][lane], red[1][lane], red[2][lane]);
 #pragma unroll
     for (int o = kThreads / 64; o > 0; o >>= 1) {
@@ -330,21 +342,22 @@ __global__ void __launch_bounds__(kThreads) token_stats_fwd_kernel(const FwdArgs
     }
   }
   __syncthreads();
-  Acc all;
+  Acc all(kt);
   all.m = total[0];
-  all.c = all.m == -INFINITY ? 0.0f : all.m * kLog2e;
+  all.c = all.m == -INFINITY ? 0.0f : all.m * kt;
   all.s = total[1];
   all.u = total[2];
   float row_max = all.m, log_s, entropy;
-  if (all.m > -kFar && all.m < kFar) {
+  if (fabsf(all.m) < kFar && fabsf(all.m) * a.inv_t < kFar && a.inv_t >= kMinInvT && a.inv_t <= kMaxInvT) {
     const float log2_s = log2f(all.s);
-    log_s = kLn2 * (log2_s - fmaf(all.m, kLog2e, -all.c));
+    log_s = kLn2 * (log2_s - fmaf(all.m, kt, -all.c));
     entropy = kLn2 * (log2_s - all.u / all.s);
   } else {  // nothing but masked tokens (or NaN), or values near the type's end: the sums about the row's own maximum
     float m = -INFINITY;
     for (int j = tid; j < a.V; j += kThreads) m = fmaxf(m, Elem<T>::one(x + j));
     row_max = block_max(m, red[0], lane, warp);
     AccExact ex;
+    ex.inv_t = a.inv_t;
     ex.m = row_max;
     for (int j = tid; j < a.V; j += kThreads) {
       const float v[1] = {Elem<T>::one(x + j)};
@@ -357,7 +370,7 @@ __global__ void __launch_bounds__(kThreads) token_stats_fwd_kernel(const FwdArgs
   }
   all.m = row_max;
   if (tid == 0) {
-    a.lp[row] = (Elem<T>::one(x + t) - all.m) - log_s;
+    a.lp[row] = fmaf(Elem<T>::one(x + t) - all.m, a.inv_t, -log_s);
     a.ent[row] = entropy;
     a.ms[2 * static_cast<long long>(row)] = all.m;
     a.ms[2 * static_cast<long long>(row) + 1] = log_s;
@@ -388,7 +401,7 @@ __global__ void __launch_bounds__(kThreads) token_stats_fwd_kernel(const FwdArgs
   auto emit = [&](int r, unsigned long long key) {
     const int idx = static_cast<int>(~static_cast<uint32_t>(key));
     top_id[r] = idx;
-    top_lp[r] = (Elem<T>::one(x + idx) - all.m) - log_s;
+    top_lp[r] = fmaf(Elem<T>::one(x + idx) - all.m, a.inv_t, -log_s);
   };
   if (n <= kMaxCand) {  // rank of each candidate among all (the keys are distinct)
     if (tid < n) {
@@ -428,6 +441,7 @@ struct BwdArgs {
   const int64_t* targets;
   int64_t ignore;
   int N, V, k;
+  float inv_t;
   const float* ent;
   const float* ms;
   const int64_t* top_id;
@@ -465,10 +479,12 @@ __global__ void __launch_bounds__(kThreads) token_stats_bwd_kernel(const BwdArgs
   float pull = fmaf(g_ent, a.ent[row], g_lp);
   if (g_top != nullptr)
     for (int i = 0; i < a.k; ++i) pull += g_top[i];
-  // -p (pull + g_ent log p); the floor keeps 0 * -inf out (see Acc::add)
+  // -p (pull + g_ent log p) / T; the floor keeps 0 * -inf out (see Acc::add)
+  const float inv_t = a.inv_t, ge = g_ent * inv_t;
+  pull *= inv_t;
   auto dense = [&](float v) {
-    const float y = max_nan((v - m) - log_s, -1e30f);
-    return -ex2_mufu(y * kLog2e) * fmaf(g_ent, y, pull);
+    const float y = max_nan(fmaf(v - m, inv_t, -log_s), -1e30f);
+    return -ex2_mufu(y * kLog2e) * fmaf(ge, y, pull);
   };
   // input vectors line up with the output's when both rows start at the same offset
   const bool aligned = ((reinterpret_cast<uintptr_t>(x) ^ reinterpret_cast<uintptr_t>(g)) & 15) == 0;
@@ -506,7 +522,7 @@ __global__ void __launch_bounds__(kThreads) token_stats_bwd_kernel(const BwdArgs
       float hot = idx == t ? g_lp : 0.0f;
       if (g_top != nullptr)
         for (int i = 0; i < a.k; ++i) hot += ids[i] == idx ? g_top[i] : 0.0f;
-      g[idx] = Elem<T>::round(hot + dense(Elem<T>::one(x + idx)));
+      g[idx] = Elem<T>::round(fmaf(hot, inv_t, dense(Elem<T>::one(x + idx))));
     }
   }
 }
@@ -528,12 +544,19 @@ const float* opt_f32(const c10::optional<torch::Tensor>& t, int64_t numel, const
   return t->data_ptr<float>();
 }
 
+float inverse(double temperature) {
+  TT_CHECK(temperature > 0 && std::isfinite(temperature) && std::isfinite(static_cast<float>(1.0 / temperature)) &&
+               static_cast<float>(1.0 / temperature) > 0,
+           "token_stats: temperature must be positive and finite");
+  return static_cast<float>(1.0 / temperature);
+}
+
 }  // namespace stats
 
 // logits [N, V] (bf16 or fp32, any row stride), targets int64 [N] -> lp, ent fp32 [N], ms fp32 [N, 2],
-// top_lp fp32 / top_id int64 [N, k].  Rows whose target is ignore_index are not scored.
-void token_stats_fwd(torch::Tensor logits, torch::Tensor targets, int64_t k, int64_t ignore_index, torch::Tensor lp,
-                     torch::Tensor ent, torch::Tensor ms, torch::Tensor top_lp, torch::Tensor top_id) {
+// top_lp fp32 / top_id int64 [N, k] of softmax(logits / temperature).  Rows whose target is ignore_index are not scored.
+void token_stats_fwd(torch::Tensor logits, torch::Tensor targets, int64_t k, int64_t ignore_index, double temperature,
+                     torch::Tensor lp, torch::Tensor ent, torch::Tensor ms, torch::Tensor top_lp, torch::Tensor top_id) {
   using namespace stats;
   check_logits(logits, targets, k);
   const int64_t N = logits.size(0), V = logits.size(1);
@@ -546,7 +569,7 @@ void token_stats_fwd(torch::Tensor logits, torch::Tensor targets, int64_t k, int
   if (N == 0) return;
   const c10::cuda::CUDAGuard guard(logits.device());
   FwdArgs a{logits.data_ptr(), logits.stride(0), targets.data_ptr<int64_t>(), ignore_index, static_cast<int>(N),
-            static_cast<int>(V), static_cast<int>(k), lp.data_ptr<float>(), ent.data_ptr<float>(), ms.data_ptr<float>(),
+            static_cast<int>(V), static_cast<int>(k), inverse(temperature), lp.data_ptr<float>(), ent.data_ptr<float>(), ms.data_ptr<float>(),
             top_lp.data_ptr<float>(), top_id.data_ptr<int64_t>(), device_status_ptr(logits.get_device())};
   if (logits.scalar_type() == torch::kBFloat16)
     token_stats_fwd_kernel<__nv_bfloat16><<<static_cast<unsigned>(N), kThreads, 0, cur_stream()>>>(a);
@@ -556,8 +579,8 @@ void token_stats_fwd(torch::Tensor logits, torch::Tensor targets, int64_t k, int
 }
 
 // grad [N, V] (contiguous, the logits' type) of sum g_lp lp + g_ent ent + g_top top_lp.
-void token_stats_bwd(torch::Tensor logits, torch::Tensor targets, int64_t k, int64_t ignore_index, torch::Tensor ent,
-                     torch::Tensor ms, torch::Tensor top_id, c10::optional<torch::Tensor> g_lp,
+void token_stats_bwd(torch::Tensor logits, torch::Tensor targets, int64_t k, int64_t ignore_index, double temperature,
+                     torch::Tensor ent, torch::Tensor ms, torch::Tensor top_id, c10::optional<torch::Tensor> g_lp,
                      c10::optional<torch::Tensor> g_ent, c10::optional<torch::Tensor> g_top, torch::Tensor grad) {
   using namespace stats;
   check_logits(logits, targets, k);
@@ -572,7 +595,7 @@ void token_stats_bwd(torch::Tensor logits, torch::Tensor targets, int64_t k, int
   if (N == 0) return;
   const c10::cuda::CUDAGuard guard(logits.device());
   BwdArgs a{logits.data_ptr(), logits.stride(0), targets.data_ptr<int64_t>(), ignore_index, static_cast<int>(N),
-            static_cast<int>(V), static_cast<int>(k), ent.data_ptr<float>(), ms.data_ptr<float>(),
+            static_cast<int>(V), static_cast<int>(k), inverse(temperature), ent.data_ptr<float>(), ms.data_ptr<float>(),
             top_id.data_ptr<int64_t>(), opt_f32(g_lp, N, "g_lp"), opt_f32(g_ent, N, "g_ent"),
             k > 0 ? opt_f32(g_top, N * k, "g_top") : nullptr, grad.data_ptr()};
   if (logits.scalar_type() == torch::kBFloat16)

@@ -1,8 +1,15 @@
 """Edges of the ragged operators on the host: ids of near ties and NaN, bad offsets and entries, the cache's states
 after an error, arguments that lie elsewhere."""
 import math
+
+import pytest
 import torch
+
+import ragged_oracle as oracle
 from tinytron_b200 import ops
+from tinytron_b200.inference import InferenceEngine
+from tinytron_b200.models import GPT, ModelConfig
+from tinytron_b200.rl import group_advantages, make_ragged_rollout, ragged_grpo_loss
 
 
 # ----------------------------------------------------------------------------- token statistics
@@ -19,3 +26,46 @@ def test_token_stats_ids_follow_the_logits():
     assert st.top_ids.tolist() == [[40, 20, 10, 0], [7, 0, 1, 2], [6, 0, 1, 2], [1, 2, 0, 3]]
     last = ops.token_stats(x[1:2, :20], torch.tensor([7]), top_k=20).top_ids[0]
     assert int(last[-1]) == 3
+
+
+def test_token_stats_temperature():
+    """Log-probs, entropy, alternatives and gradients of softmax(logits / T)."""
+    g = torch.Generator().manual_seed(5)
+    x = torch.randn(6, 300, generator=g).mul(3)
+    t = torch.randint(0, 300, (6,), generator=g)
+    t[2] = -100
+    for temp in (0.7, 2.5):
+        leaf = x.clone().requires_grad_(True)
+        st = ops.token_stats(leaf, t, top_k=3, temperature=temp)
+        z = x.double() / temp
+        lp, ent, tops, ids, _ = oracle.token_stats(z, t, 3)
+        assert torch.equal(st.top_ids, ids)
+        for a, b in ((st.log_probs, lp), (st.entropy, ent), (st.top_log_probs, tops)):
+            assert torch.allclose(a.double(), b, atol=1e-5)
+        ga, gb, gc = torch.randn(6, generator=g), torch.randn(6, generator=g), torch.randn(6, 3, generator=g)
+        (grad,) = torch.autograd.grad([st.log_probs, st.entropy, st.top_log_probs], leaf, [ga, gb, gc])
+        want, _ = oracle.token_stats_grad(z, t, ga, gb, gc, ids)
+        assert torch.allclose(grad.double(), want / temp, atol=1e-5)
+    for bad in (0.0, -1.0, math.nan, math.inf):
+        with pytest.raises(ValueError):
+            ops.token_stats(x, t, temperature=bad)
+
+
+def test_policy_ratio_is_one_at_a_temperature():
+    """The actor is the sampler at T != 1 too."""
+    c = cfg()
+    eng = InferenceEngine(c, device="cpu", dtype=torch.float32, kv_cache_page_size=4)
+    torch.manual_seed(1)
+    gen = eng.generate_ragged([torch.tensor([3, 4, 5]), torch.tensor([6])], 6, num_samples=3, temperature=0.6)
+    actor = GPT(c, device="cpu")
+    actor.load_state_dict(eng.model.state_dict())
+    out = ragged_grpo_loss(actor, make_ragged_rollout(gen), group_advantages(torch.arange(6.0), 3), temperature=0.6)
+    assert abs(float(out.metrics["mean_ratio"]) - 1) < 1e-4 and float(out.metrics["clip_frac"]) == 0
+
+
+# ----------------------------------------------------------------------------- offsets and entries
+def cfg(**kw):
+    base = dict(block_size=128, vocab_size=120, num_layer=2, num_attention_heads=4, num_key_value_heads=2, hidden_size=64,
+                intermediate_size=96, init_std=0.05, seed=3)
+    base.update(kw)
+    return ModelConfig(**base)

@@ -119,3 +119,81 @@ def test_packed_attention_unseen_values_weigh_nothing(d):
         got = run_packed(q, k, bad, do, cu_of(lens))
         for x, y in zip(got[:2], clean[:2]):
             assert torch.equal(x[:40 + at], y[:40 + at]) and torch.equal(x[240:], y[240:])
+
+
+# ----------------------------------------------------------------------------- token statistics
+def check_tempered(x, t, top, temp):
+    z = x.double() / temp
+    leaf = x.detach().requires_grad_(True)
+    st = ops().token_stats(leaf, t, top_k=top, temperature=temp)
+    lp, ent, tops, _, y = oracle.token_stats(z, t, top)
+    ids = torch.sort(x.double(), dim=-1, descending=True, stable=True).indices[:, :top]
+    assert torch.equal(st.top_ids, torch.where((t != -100)[:, None], ids, torch.full_like(ids, -1)))
+    # a scaled difference d is off by a few roundings of itself (1 / T, log2 e / T, the product): 2^-21 |d|
+    d = (z - z.amax(-1, keepdim=True)).abs()
+    near = d.gather(1, t.clamp_min(0)[:, None])[:, 0]
+    scored = (t != -100).double()
+    within(st.log_probs, lp, scored * (1e-5 + 2.0 ** -21 * near + 2.0 ** -21 * lp.abs()), "log-probs")
+    within(st.entropy, ent, 4e-5 * (1 + ent), "entropy")
+    within(st.top_log_probs, tops, 1e-5 + 2.0 ** -20 * tops.abs(), "top")
+    g = gen(9)
+    n = x.shape[0]
+    ga, gb, gc = randn(g, n, dtype=torch.float32), randn(g, n, dtype=torch.float32), randn(g, n, top, dtype=torch.float32)
+    (grad,) = torch.autograd.grad([st.log_probs, st.entropy, st.top_log_probs], leaf, [ga, gb, gc])
+    want, mag = oracle.token_stats_grad(z, t, ga, gb, gc, ids)
+    far = torch.where(y.isfinite(), y.abs(), torch.zeros_like(y))  # a probability is off by its exponent's error
+    tol = (3e-5 + 2.0 ** -20 * far) * mag / temp + (2.0 ** -8 * want.abs() / temp if x.dtype == torch.bfloat16 else 0)
+    within(grad, want / temp, tol + 1e-30, "gradient")
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("temp", [0.7, 1.3, 0.05, 30.0, 1e-4, 1e4])
+def test_token_stats_temperature(dtype, temp):
+    g = gen(11)
+    x = randn(g, 8, 3001, dtype=torch.float32).mul(3)
+    x[1, ::3] = -math.inf
+    x[2, 9:] = torch.finfo(dtype).min
+    x[3] += 500.0
+    x[4] = 1.25
+    x = x.to(dtype)
+    t = torch.tensor([5, 1, 3, 2999, 17, -100, 0, 3000], device=DEV)
+    check_tempered(x, t, 5, temp)
+
+
+@pytest.mark.parametrize("temp", [0.7, 1.4])
+def test_token_stats_scores_what_the_sampler_drew(temp):
+    """Log-prob of the drawn tokens under the distribution they were drawn from, from the same bf16 logits."""
+    from tinytron_b200.inference.sampler import sample_next_token_with_log_prob
+
+    torch.manual_seed(3)
+    x = randn(gen(12), 64, 8000).mul_(2.5)
+    tok, lp = sample_next_token_with_log_prob(x, temp)
+    st = ops().token_stats(x, tok, temperature=temp)
+    assert float((st.log_probs - lp).abs().max()) < 1e-4
+
+
+def test_packed_scores_at_a_temperature_round_the_logits_once(monkeypatch):
+    """packed_token_stats at T != 1 is log softmax(logits / T) of the LM head's own logits."""
+    from tinytron_b200.models import GPT, ModelConfig
+
+    c = ModelConfig(block_size=512, vocab_size=512, num_layer=1, num_attention_heads=4, num_key_value_heads=2, hidden_size=256,
+                    intermediate_size=512, init_std=0.2, seed=5)
+    m = GPT(c, device=DEV)
+    g = torch.Generator().manual_seed(0)
+    idx = torch.randint(0, 512, (300,), generator=g).to(DEV)
+    labels = torch.randint(0, 512, (300,), generator=g).to(DEV)
+    real, seen = ops().linear, []
+
+    def linear(x, *w):
+        y = real(x, *w)
+        if w[0] is m.lm_head.weight:
+            seen.append(y.detach())
+        return y
+
+    monkeypatch.setattr(ops(), "linear", linear)
+    with torch.no_grad():
+        st = m.packed_token_stats(idx, labels, i32([0, 100, 300]), temperature=0.7)
+    assert len(seen) == 1 and seen[0].dtype == torch.bfloat16
+    want = torch.log_softmax(seen[0].double() / 0.7, -1).gather(1, labels[:, None])[:, 0]
+    assert float(want.abs().max()) > 1
+    within(st.log_probs, want, 1e-4 + 2.0 ** -20 * want.abs(), "log-probs")

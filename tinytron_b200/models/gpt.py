@@ -167,7 +167,7 @@ class GPT(nn.Module):
     def packed_token_stats(self, idx, targets, cu_seqlens, top_k: int = 0, max_seqlen: int | None = None,
                            temperature: float = 1.0):
         """Statistics (:class:`~tinytron_b200.ops.TokenStats`, differentiable) of ``targets`` [N] under the model's
-        next-token distributions over sequences packed end to end: ``idx`` [N], ``cu_seqlens`` int32 [S + 1].
+        next-token distributions at ``temperature`` over sequences packed end to end: ``idx`` [N], ``cu_seqlens`` int32 [S + 1].
         Targets equal to the ignore index (-100) are not scored."""
         x = ops.embedding(idx, self.wte.weight)
         pending = None
@@ -179,9 +179,7 @@ class GPT(nn.Module):
             pending = (out[0] if self.use_moe else out).squeeze(0)
         _, h = ops.add_rmsnorm(x, pending, self.lnf.weight, self.eps)
         logits = ops.linear(h, self.lm_head.weight)
-        if temperature != 1.0:
-            logits = logits / temperature
-        return ops.token_stats(logits, targets, top_k, self.loss_fn.ignore_index)
+        return ops.token_stats(logits, targets, top_k, self.loss_fn.ignore_index, temperature)
 
     def forward_ragged(self, idx, step, rows=None):
         """Logits [N, V] (of ``rows`` only, if given) of the tokens ``idx`` [N] of one

@@ -411,12 +411,12 @@ class TokenStats(NamedTuple):
     top_ids: torch.Tensor
 
 
-def _token_stats_fwd(logits, targets, top_k, ignore_index):
+def _token_stats_fwd(logits, targets, top_k, ignore_index, temperature):
     n = logits.shape[0]
     f = dict(dtype=torch.float32, device=logits.device)
     lp, ent, ms, top = torch.empty(n, **f), torch.empty(n, **f), torch.empty(n, 2, **f), torch.empty(n, top_k, **f)
     ids = torch.empty(n, top_k, dtype=torch.long, device=logits.device)
-    _C().token_stats_fwd(logits, targets, top_k, ignore_index, lp, ent, ms, top, ids)
+    _C().token_stats_fwd(logits, targets, top_k, ignore_index, temperature, lp, ent, ms, top, ids)
     return lp, ent, top, ids, ms
 
 
@@ -424,10 +424,10 @@ class TokenStatsFn(torch.autograd.Function):
     """One pass over the logits forward, one read and one write backward (csrc/fused/token_stats.cu)."""
 
     @staticmethod
-    def forward(ctx, logits, targets, top_k, ignore_index):
-        lp, ent, top, ids, ms = _token_stats_fwd(logits, targets, top_k, ignore_index)
+    def forward(ctx, logits, targets, *cfg):
+        lp, ent, top, ids, ms = _token_stats_fwd(logits, targets, *cfg)
         ctx.save_for_backward(logits, targets, ent, ms, ids)
-        ctx.cfg = (top_k, ignore_index)
+        ctx.cfg = cfg  # top_k, ignore_index, temperature
         ctx.set_materialize_grads(False)
         ctx.mark_non_differentiable(ids)
         return lp, ent, top, ids
@@ -439,7 +439,7 @@ class TokenStatsFn(torch.autograd.Function):
         grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
         g = [x.float().contiguous() if x is not None else None for x in (g_lp, g_ent, g_top)]
         _C().token_stats_bwd(logits, targets, *ctx.cfg, ent, ms, ids, *g, grad)
-        return grad, None, None, None
+        return grad, None, None, None, None
 
 
 def _ranking(x):
@@ -451,14 +451,14 @@ def _ranking(x):
     return order.gather(1, last)
 
 
-def _token_stats_cpu(logits, targets, top_k, ignore_index):
+def _token_stats_cpu(logits, targets, top_k, ignore_index, temperature):
     scored = targets != ignore_index
     t = targets.clamp(min=0)
     if bool((scored & ((targets < 0) | (targets >= logits.shape[-1]))).any()):
         raise ValueError("a target is outside the vocabulary")
     zero = torch.zeros((), dtype=torch.float32)
     # rows that are not scored must not reach the gradient, whatever they hold
-    y = torch.log_softmax(torch.where(scored[:, None], logits.float(), zero), -1)
+    y = torch.log_softmax(torch.where(scored[:, None], logits.float() / temperature, zero), -1)
     lp = torch.where(scored, y.gather(1, t[:, None])[:, 0], zero)
     p = y.exp()
     ent = torch.where(scored, -(p * torch.where(p > 0, y, zero)).sum(-1), zero)  # p log p is 0 where p is
@@ -467,8 +467,9 @@ def _token_stats_cpu(logits, targets, top_k, ignore_index):
     return lp, ent, top, torch.where(scored[:, None], ids, torch.full_like(ids, -1))
 
 
-def token_stats(logits: torch.Tensor, targets: torch.Tensor, top_k: int = 0, ignore_index: int = IGNORE_INDEX) -> TokenStats:
-    """Statistics of given tokens under softmax(logits), in fp32 and differentiable in the logits.
+def token_stats(logits: torch.Tensor, targets: torch.Tensor, top_k: int = 0, ignore_index: int = IGNORE_INDEX,
+                temperature: float = 1.0) -> TokenStats:
+    """Statistics of given tokens under softmax(logits / temperature), in fp32 and differentiable in the logits.
 
     logits [..., V] bf16 or fp32 (rows contiguous; a row stride of its own is fine), targets [...] int64.  Rows whose
     target is ``ignore_index`` are not scored: log-prob, entropy and alternatives 0, ids -1, no gradient.  The ``top_k``
@@ -483,6 +484,9 @@ def token_stats(logits: torch.Tensor, targets: torch.Tensor, top_k: int = 0, ign
         raise ValueError(f"top_k must be between 0 and min({MAX_TOP_K}, {v}), got {top_k}")
     if logits.dtype not in (torch.bfloat16, torch.float32):
         raise ValueError(f"logits must be bfloat16 or float32, got {logits.dtype}")
+    temperature = float(temperature)
+    if not (temperature > 0 and math.isfinite(temperature)):
+        raise ValueError(f"temperature must be positive and finite, got {temperature}")
     lead = tuple(targets.shape)
     x = logits.reshape(-1, v)
     t = targets.reshape(-1).contiguous()
@@ -490,9 +494,9 @@ def token_stats(logits: torch.Tensor, targets: torch.Tensor, top_k: int = 0, ign
         if v and x.stride(-1) != 1:
             x = x.contiguous()
         if torch.is_grad_enabled() and x.requires_grad:
-            lp, ent, top, ids = TokenStatsFn.apply(x, t, top_k, ignore_index)
+            lp, ent, top, ids = TokenStatsFn.apply(x, t, top_k, ignore_index, temperature)
         else:
-            lp, ent, top, ids, _ = _token_stats_fwd(x, t, top_k, ignore_index)
+            lp, ent, top, ids, _ = _token_stats_fwd(x, t, top_k, ignore_index, temperature)
     else:
-        lp, ent, top, ids = _token_stats_cpu(x, t, top_k, ignore_index)
+        lp, ent, top, ids = _token_stats_cpu(x, t, top_k, ignore_index, temperature)
     return TokenStats(lp.view(lead), ent.view(lead), top.view(*lead, top_k), ids.view(*lead, top_k))
