@@ -197,3 +197,33 @@ def test_packed_scores_at_a_temperature_round_the_logits_once(monkeypatch):
     want = torch.log_softmax(seen[0].double() / 0.7, -1).gather(1, labels[:, None])[:, 0]
     assert float(want.abs().max()) > 1
     within(st.log_probs, want, 1e-4 + 2.0 ** -20 * want.abs(), "log-probs")
+
+
+# ----------------------------------------------------------------------------- gradients that the kernels do not have
+def test_serving_operators_refuse_to_lose_gradients():
+    from tinytron_b200.inference import RaggedKVCache
+    from tinytron_b200.models import GPT, ModelConfig
+    from tinytron_b200.ops.rope import rope_tables
+
+    g = gen(13)
+    kp, vp = randn(g, 4, 16, 2, 64), randn(g, 4, 16, 2, 64)
+    q, table, n = randn(g, 1, 4, 64), i32([[0, 1]]), i32([20])
+    for i in range(3):
+        args = [q, kp, vp]
+        args[i] = args[i].clone().requires_grad_(True)
+        with pytest.raises(ValueError, match="gradient"):
+            ops().paged_attention(*args, table, n)
+        with torch.no_grad():
+            ops().paged_attention(*args, table, n)
+    qkv = randn(g, 3, 8 * 64).requires_grad_(True)
+    cos, sin = rope_tables(64, 10000.0, 64, DEV)
+    with pytest.raises(ValueError, match="gradient"):
+        ops().rotary_append(qkv, cos, sin, 4, 2, i32([0, 3]))
+    with torch.no_grad():
+        ops().rotary_append(qkv, cos, sin, 4, 2, i32([0, 3]))
+    c = ModelConfig(block_size=64, vocab_size=128, num_layer=1, num_attention_heads=4, num_key_value_heads=2, hidden_size=256,
+                    intermediate_size=256, seed=5)
+    model, cache = GPT(c, device=DEV), RaggedKVCache.from_model_config(c, 4, 16, 2, DEV, torch.bfloat16)
+    (s,) = cache.add()
+    step = cache.prefill_step([s], [5])
+    assert not model.forward_ragged(torch.arange(5, device=DEV), step).requires_grad

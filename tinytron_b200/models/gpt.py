@@ -181,9 +181,11 @@ class GPT(nn.Module):
         logits = ops.linear(h, self.lm_head.weight)
         return ops.token_stats(logits, targets, top_k, self.loss_fn.ignore_index, temperature)
 
+    @torch.no_grad()
     def forward_ragged(self, idx, step, rows=None):
         """Logits [N, V] (of ``rows`` only, if given) of the tokens ``idx`` [N] of one
-        :class:`~tinytron_b200.inference.ragged.RaggedStep`; their keys and values are appended to its cache."""
+        :class:`~tinytron_b200.inference.ragged.RaggedStep`; their keys and values are appended to its cache.  No
+        gradient: the cached keys and values have none (``packed_token_stats`` scores with one)."""
         x = ops.embedding(idx, self.wte.weight)
         pending = None
         for blk in self.blocks:

@@ -43,6 +43,13 @@ def _heads(name: str, t: torch.Tensor, dtype, device, tokens: int | None = None,
         raise ValueError(f"{name} must be {dtype} on {device}, got {t.dtype} on {t.device}")
 
 
+def _no_gradient(op: str, *inputs: torch.Tensor) -> None:
+    """The serving kernels record no gradient: refuse inputs whose gradient would silently stop here."""
+    if torch.is_grad_enabled() and any(x.requires_grad for x in inputs):
+        raise ValueError(f"{op} has no gradient on CUDA and its inputs require one: call it under torch.no_grad()"
+                         + (" (rotary_packed_attention is differentiable)" if op == "rotary_append" else ""))
+
+
 def _kernel_rows(t: torch.Tensor) -> torch.Tensor:
     """``t`` itself where the kernels can read it in place (head rows contiguous, 16-byte aligned strides),
     else a contiguous copy."""
@@ -218,7 +225,7 @@ def rotary_append(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, num_h
     position ``start[b]`` (0 without ``start``; one token per sequence is ``cu_seqlens = arange(B + 1)``).
     cos/sin fp32 [max_pos, D / 2] (``rope_tables``).  With pools [pages, page_size, Hkv, D] and ``page_table`` int32
     [B, width], token t goes to page ``page_table[b, t // page_size]``.  Returns (q [N, Hq, D], k [N, Hkv, D] or None);
-    rows of no sequence come back as zeros and are written nowhere."""
+    rows of no sequence come back as zeros and are written nowhere.  No gradient on CUDA (refused where one is wanted)."""
     d = 2 * cos.shape[1]
     n = qkv.shape[0]
     if qkv.dim() != 2 or qkv.shape[1] < (num_heads + 2 * num_kv_heads) * d:
@@ -233,6 +240,7 @@ def rotary_append(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, num_h
         _pool("rotary_append", k_pages, v_pages, (4,))
         _int32("page_table", page_table, qkv.device, 2)
     if qkv.is_cuda:
+        _no_gradient("rotary_append", qkv)
         q = torch.empty(n, num_heads, d, dtype=qkv.dtype, device=qkv.device)
         k = torch.empty(n, num_kv_heads, d, dtype=qkv.dtype, device=qkv.device) if want_k else None
         _C().rotary_append(qkv, cos, sin, num_heads, num_kv_heads, d, cu, start, False, q, k, k_pages, v_pages, page_table)
@@ -366,7 +374,8 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     q [B, Hq, D] bf16 (D 64 or 128, up to 16 query heads per kv head), pools [pages, page_size, Hkv, D] with any page
     size, ``page_table`` int32 [B, width], ``seq_lens`` int32 [B]: query b attends to its first ``seq_lens[b]`` keys
     (0: output zeros).  The lengths are read on the device, so a captured call replays with new ones.
-    ``workspace`` (:func:`paged_attention_workspace`) is taken from a per-stream cache if not given."""
+    ``workspace`` (:func:`paged_attention_workspace`) is taken from a per-stream cache if not given.  No gradient on
+    CUDA (refused where one is wanted)."""
     _pool("paged_attention", k_pages, v_pages, (4,))
     _heads("q", q, k_pages.dtype, k_pages.device, dim=k_pages.shape[3])
     _int32("page_table", page_table, q.device, 2)
@@ -382,6 +391,7 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
         if q.dtype != torch.bfloat16 or d not in (64, 128) or hq // hkv > 16:
             raise ValueError(f"paged_attention runs bf16, head_dim 64 or 128 and up to 16 query heads per kv head on CUDA, got "
                              f"{q.dtype}, {d} and {hq // hkv}")
+        _no_gradient("paged_attention", q, k_pages, v_pages)
         out = torch.empty(b, hq, d, dtype=q.dtype, device=q.device)
         ws = workspace if workspace is not None else _stream_workspace(q, k_pages, page_table)
         _C().paged_attention(_kernel_rows(q), k_pages, v_pages, page_table, seq_lens, scale, ws.partials, ws.counters, out)
