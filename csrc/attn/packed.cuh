@@ -64,6 +64,21 @@ __device__ __forceinline__ int query_tiles(const Seq& s, bool extra, int kt) {
   return max(0, (s.qlen + kBlock - 1) / kBlock - first_query_tile(s, kt));
 }
 
+// Sequence of a list entry past the end of the list, and of every entry where the offsets are unusable.
+constexpr int kNoEntry = -1, kRejected = -2;
+
+// This block's share of zeros for a [tokens, heads, D] tensor with strides (elements): the output of a call whose
+// offsets are unusable.
+template <int D>
+__device__ __forceinline__ void zero_share(__nv_bfloat16* t, long long tokens, int heads, long long ld_n, long long ld_h) {
+  constexpr int NU = D / 8;
+  const long long all = tokens * heads * NU, step = static_cast<long long>(gridDim.x) * blockDim.x;
+  for (long long i = static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x; i < all; i += step) {
+    const long long row = i / NU;
+    reinterpret_cast<uint4*>(t + row / heads * ld_n + row % heads * ld_h)[i % NU] = make_uint4(0u, 0u, 0u, 0u);
+  }
+}
+
 // Zeroes rows [from, 128) of a swizzled tile of D / 64 chunks (whole 128-byte rows, so the swizzle
 // does not matter), by `threads` threads of index t.
 template <int D>
@@ -193,8 +208,9 @@ inline void allow_smem(size_t smem, int device) {
 
 enum ScheduleKind { kQueryPairs = 0, kQueryTiles = 1, kKeyTiles = 2 };
 
-// List (int2 {sequence, tile}, longest first, {-1, 0} past the end) of a packing's query tile pairs, query
-// tiles or key tiles; `capacity` entries.
+// List (int2 {sequence, tile}, longest first, {kNoEntry, 0} past the end) of a packing's query tile pairs, query
+// tiles or key tiles; `capacity` entries.  Offsets that do not ascend from 0 within the tokens: kBadIndex in the status
+// word, all entries {kRejected, 0}, and the kernels that read the list write zeros.
 void schedule(const Packing& p, ScheduleKind kind, int2* list, int capacity, int* status, cudaStream_t stream);
 
 }  // namespace packed

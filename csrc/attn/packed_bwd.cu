@@ -202,7 +202,13 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
   constexpr uint32_t S_COL = 0, DP_COL = kBlock, DV_COL = 2 * kBlock, DK_COL = 2 * kBlock + D;
   constexpr uint32_t TMEM_COLS = 512;
   const int2 entry = p.list[blockIdx.x / p.Hkv];
-  if (entry.x < 0) return;
+  if (entry.x < 0) {
+    if (entry.x == kRejected) {
+      zero_share<D>(p.d0, p.pk.Nk, p.Hkv, p.d0_n, p.d0_h);
+      zero_share<D>(p.d1, p.pk.Nk, p.Hkv, p.d1_n, p.d1_h);
+    }
+    return;
+  }
   const int g = static_cast<int>(blockIdx.x) % p.Hkv;
   const int group = p.Hq / p.Hkv;
   const Seq s = sequence(p.pk, entry.x);
@@ -433,7 +439,10 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
   constexpr uint32_t DP_COL = 2 * kBlock, DQ_COL = 3 * kBlock;
   constexpr uint32_t TMEM_COLS = 512;
   const int2 entry = p.list[blockIdx.x / p.Hq];
-  if (entry.x < 0) return;
+  if (entry.x < 0) {
+    if (entry.x == kRejected) zero_share<D>(p.d0, p.pk.Nq, p.Hq, p.d0_n, p.d0_h);
+    return;
+  }
   const int h = static_cast<int>(blockIdx.x) % p.Hq;
   const int g = h / (p.Hq / p.Hkv);
   const Seq s = sequence(p.pk, entry.x);
@@ -688,7 +697,7 @@ void packed_attn_bwd(torch::Tensor q, torch::Tensor k, torch::Tensor v, torch::T
   p.status = status;
   const CUtensorMap tq = head_map_3d(q, kBlock, "q"), tk = head_map_3d(k, kBlock, "k"), tv = head_map_3d(v, kBlock, "v"),
                     tdo = head_map_3d(dout, kBlock, "dout");
-  // dQ's list first: it checks the offsets, and a bad packing leaves every entry empty
+  // dQ's list first: it checks the offsets, and a bad packing leaves every entry rejected
   schedule(p.pk, kQueryTiles, list, static_cast<int>(q_entries), status, st);
   packed_stats_kernel<<<static_cast<unsigned>(pad_slots(Nq, B) * (kBlock / kStatsRows)), 256, 0, st>>>(
       p.pk, list, reinterpret_cast<const __nv_bfloat16*>(o.data_ptr()), reinterpret_cast<const __nv_bfloat16*>(o_lo.data_ptr()),

@@ -63,7 +63,7 @@ __global__ void __launch_bounds__(kSchedThreads) schedule_kernel(const Packing p
   __syncthreads();
   if (bad) {  // nothing is computed
     if (tid == 0) atomicCAS(status, 0, static_cast<int>(kBadIndex));
-    for (int i = tid; i < capacity; i += kSchedThreads) list[i] = make_int2(-1, 0);
+    for (int i = tid; i < capacity; i += kSchedThreads) list[i] = make_int2(kRejected, 0);
     return;
   }
   constexpr int kWarps = kSchedThreads / 32;
@@ -97,7 +97,7 @@ __global__ void __launch_bounds__(kSchedThreads) schedule_kernel(const Packing p
       if (at < capacity) list[at] = make_int2(b, t);
     }
   }
-  for (int i = total + tid; i < capacity; i += kSchedThreads) list[i] = make_int2(-1, 0);
+  for (int i = total + tid; i < capacity; i += kSchedThreads) list[i] = make_int2(kNoEntry, 0);
 }
 static_assert(kBins == 2 * kSchedThreads, "two bins per thread");
 
@@ -157,7 +157,17 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   const int units = p.head_pairs ? p.Hq / 2 : p.Hq;
   const int2 entry = p.list[blockIdx.x / units];
-  if (entry.x < 0) return;  // past the end of the list (uniform over the block, nothing allocated)
+  if (entry.x < 0) {  // past the end of the list (uniform over the block, nothing allocated)
+    if (entry.x == kRejected) {
+      zero_share<D>(p.o, p.pk.Nq, p.Hq, static_cast<long long>(p.Hq) * D, D);
+      if (p.o_lo != nullptr) zero_share<D>(p.o_lo, p.pk.Nq, p.Hq, static_cast<long long>(p.Hq) * D, D);
+      if (p.lse != nullptr)
+        for (long long i = static_cast<long long>(blockIdx.x) * kThreads + threadIdx.x; i < static_cast<long long>(p.Hq) * p.pk.Nq;
+             i += static_cast<long long>(gridDim.x) * kThreads)
+          p.lse[i] = -INFINITY;
+    }
+    return;
+  }
   const int h0 = static_cast<int>(blockIdx.x) % units * (p.head_pairs ? 2 : 1);
   const int g = h0 / (p.Hq / p.Hkv);
   const Seq s = sequence(p.pk, entry.x);

@@ -7,7 +7,7 @@
 // All three are bound by the bytes they move: 16-byte vectors, several in flight per thread.
 //
 // Index inputs live on the device and are checked where they are used: an entry out of range is
-// skipped and recorded as kBadIndex in the status word.
+// skipped and recorded as kBadIndex in the status word; a token at a position past the tables comes back as zeros.
 //
 // Measured (L2 flushed): appending 16384 tokens of 16/4 heads, d 128 (218 MB): 51 us, 4.3 TB/s; moving 16 KB
 // pages of 16 layers (772 MB): 123 us, 6.3 TB/s; forking 8 prompts into 8 answers each over 16 layers
@@ -64,17 +64,16 @@ __global__ void __launch_bounds__(kThreads) rotary_append_kernel(const AppendArg
   if (tok >= a.N) return;
   const int b = find_sequence(a.cu, a.B, tok, lane);
   const int c0 = a.cu[b];
-  if (tok < c0 || tok >= a.cu[b + 1]) {  // a token of no sequence: nothing is cached, zeros come back
+  const bool inside = tok >= c0 && tok < a.cu[b + 1];
+  const int pos = inside ? (a.start != nullptr ? a.start[b] : 0) + tok - c0 : 0;
+  const bool bad = pos < 0 || pos >= a.max_pos;
+  if (bad && lane == 0) atomicCAS(a.status, 0, static_cast<int>(kBadIndex));
+  if (!inside || bad) {  // a token of no sequence, or past the tables: nothing is cached, zeros come back
     for (int i = lane; i < a.Hq * a.D / 8; i += 32)
       reinterpret_cast<uint4*>(a.q_out + static_cast<long long>(tok) * a.ld_q)[i] = make_uint4(0u, 0u, 0u, 0u);
     if (a.k_out != nullptr)
       for (int i = lane; i < a.Hkv * a.D / 8; i += 32)
         reinterpret_cast<uint4*>(a.k_out + static_cast<long long>(tok) * a.ld_k)[i] = make_uint4(0u, 0u, 0u, 0u);
-    return;
-  }
-  const int pos = (a.start != nullptr ? a.start[b] : 0) + tok - c0;
-  if (pos < 0 || pos >= a.max_pos) {
-    if (lane == 0) atomicCAS(a.status, 0, static_cast<int>(kBadIndex));
     return;
   }
   long long slot = -1;  // the token's row of heads in a page

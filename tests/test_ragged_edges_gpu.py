@@ -10,6 +10,7 @@ import ragged_oracle as oracle
 pytestmark = pytest.mark.gpu
 
 DEV = "cuda"
+K_BAD_INDEX = 8
 
 
 def ops():
@@ -50,6 +51,12 @@ def within(got, want, tol, what):
     assert got.shape == want.shape, (what, got.shape, want.shape)
     bad = ~((got.double() - want).abs() <= tol)
     assert not bool(bad.any()), (what, int(bad.sum()), float((got.double() - want).abs().max()))
+
+
+def dirty_memory(mb=64):
+    """Freed blocks full of NaN: what torch.empty returns next is not zero by luck."""
+    blocks = [torch.full((n,), math.nan, device=DEV) for n in (64, 1024, 65536, 1 << 20, mb << 18) for _ in range(8 if n < 1 << 20 else 1)]
+    del blocks
 
 
 @pytest.fixture(autouse=True)
@@ -227,3 +234,48 @@ def test_serving_operators_refuse_to_lose_gradients():
     (s,) = cache.add()
     step = cache.prefill_step([s], [5])
     assert not model.forward_ragged(torch.arange(5, device=DEV), step).requires_grad
+
+
+# ----------------------------------------------------------------------------- rejected entries
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("cu", [[0, 301], [1, 300], [0, 200, 150, 300], [0, -2, 300]], ids=str)
+def test_packed_attention_with_bad_offsets_gives_zeros(cu, d):
+    q, k, v, do = packed_inputs([300], 4, 2, d, seed=4)
+    dirty_memory()
+    qkv = torch.cat([q, k, v], 1)  # gradients of views too
+    got = run_packed(q, k, v, do, cu)
+    assert status_and_clear() == K_BAD_INDEX
+    for x in got:
+        assert bool((x == 0).all())
+    leaf = qkv.view(300, -1).clone().requires_grad_(True)
+    dirty_memory()
+    o = ops().rotary_packed_attention(leaf * 1, i32(cu), 4, 2, d)
+    (grad,) = torch.autograd.grad(o, leaf, do.view(300, -1))
+    assert status_and_clear() == K_BAD_INDEX
+    assert bool((o == 0).all()) and bool((grad == 0).all())
+
+
+def test_rotary_append_gives_zeros_at_bad_positions_and_the_rest_right():
+    from tinytron_b200.ops.rope import rope_tables
+
+    hq, hkv, d, page = 2, 1, 64, 16
+    qkv = randn(gen(5), 9, (hq + 2 * hkv) * d)
+    cos, sin = rope_tables(d, 10000.0, 64, DEV)
+    cos, sin = cos[:64].contiguous(), sin[:64].contiguous()
+    kp = torch.zeros(8, page, hkv, d, dtype=torch.bfloat16, device=DEV)
+    vp = torch.zeros_like(kp)
+    table = i32([[0, 1, 2, 3], [4, 5, -1, -1], [6, -1, -1, -1]])
+    want = ops().rotary_append(qkv, cos, sin, hq, hkv, i32([0, 3, 6, 9]), i32([62, 4, 0]), want_k=True)
+    assert status_and_clear() == K_BAD_INDEX  # the third token of the first sequence is at position 64
+    dirty_memory()
+    q, k = ops().rotary_append(qkv, cos, sin, hq, hkv, i32([0, 3, 6, 9]), i32([62, 4, 15]), kp, vp, table)
+    assert status_and_clear() == K_BAD_INDEX
+    assert bool((q[2] == 0).all()) and bool((k[2] == 0).all())
+    for i in (0, 1, 3, 4, 5):
+        assert torch.equal(q[i], want[0][i]) and torch.equal(k[i], want[1][i])
+    at = [(3, 14), (3, 15), None, (4, 4), (4, 5), (4, 6), (6, 15), None, None]  # the last two fall onto no page
+    kw, vw = torch.zeros_like(kp), torch.zeros_like(vp)
+    for i, where in enumerate(at):
+        if where is not None:
+            kw[where], vw[where] = k[i], qkv[i].view(-1, d)[hq + hkv:]
+    assert torch.equal(kp, kw) and torch.equal(vp, vw)

@@ -4,8 +4,10 @@ sequences have lengths of their own, and statistics of given tokens.
 As in :mod:`tinytron_b200.ops`, a CUDA input runs the sm_100a kernels and a CPU input plain
 torch math of the same definition; there is no fallback between the two.  Shapes, types and
 strides are checked on the host (``ValueError`` here, ``RuntimeError`` at the extension);
-index tensors live on the device, and an entry out of range is skipped and recorded in the
-status word that ``ops.check_status()`` raises on.
+index tensors live on the device, and an entry out of range is skipped (its output rows are
+zeros; where offsets do not ascend, all of them) and recorded in the status word that
+``ops.check_status()`` raises on: call it where the host waits for the device anyway, and before
+a step is taken on the results.
 """
 from __future__ import annotations
 
@@ -373,7 +375,8 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
 
     q [B, Hq, D] bf16 (D 64 or 128, up to 16 query heads per kv head), pools [pages, page_size, Hkv, D] with any page
     size, ``page_table`` int32 [B, width], ``seq_lens`` int32 [B]: query b attends to its first ``seq_lens[b]`` keys
-    (0: output zeros).  The lengths are read on the device, so a captured call replays with new ones.
+    (0: output zeros; recorded in the status word: a length past the table, cut there, and a key on a page that is not
+    mapped, which counts as zeros).  The lengths are read on the device, so a captured call replays with new ones.
     ``workspace`` (:func:`paged_attention_workspace`) is taken from a per-stream cache if not given.  No gradient on
     CUDA (refused where one is wanted)."""
     _pool("paged_attention", k_pages, v_pages, (4,))
