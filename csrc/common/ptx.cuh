@@ -17,7 +17,7 @@
 
 namespace tt {
 
-// Status codes written into the device status word (first writer wins).
+// Status codes written into the device status word (the first writer wins, a failed wait over a bad index).
 enum StatusCode : int {
   kOk = 0,
   kTimeoutFull = 1,     // consumer waited too long for a TMA stage
@@ -75,9 +75,19 @@ __device__ __forceinline__ bool mbar_try_wait(uint32_t bar_addr, uint32_t parity
   return ok != 0;
 }
 
+// True if a wait has failed somewhere: others need not run out too.  An index out of range (kBadIndex) cost its own
+// entry only, so kernels that run before the host looks wait as ever.
+__device__ __forceinline__ bool wait_failed(const int* status) {
+  const int code = *reinterpret_cast<const volatile int*>(status);
+  return code != kOk && code != kBadIndex;
+}
+__device__ __forceinline__ void record_failed_wait(int* status, int code) {
+  if (atomicCAS(status, static_cast<int>(kOk), code) == kBadIndex) atomicCAS(status, static_cast<int>(kBadIndex), code);
+}
+
 // Bounded wait for the phase with the given parity to complete.
 // Returns false (after recording `code` in *status) on timeout, or if another
-// thread already recorded an error.
+// thread's wait already failed.
 __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, int* status, int code) {
   const uint32_t a = smem_u32(bar);
   if (mbar_try_wait(a, parity)) return true;
@@ -86,9 +96,9 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, int* s
   while (true) {
     if (mbar_try_wait(a, parity)) return true;
     if ((++spins & 255u) == 0u) {
-      if (*reinterpret_cast<volatile int*>(status) != 0) return false;
+      if (wait_failed(status)) return false;
       if (globaltimer() - t0 > TT_WAIT_TIMEOUT_NS) {
-        atomicCAS(status, 0, code);
+        record_failed_wait(status, code);
         return false;
       }
     }
@@ -318,9 +328,9 @@ __device__ __forceinline__ bool mbar_wait_cluster(uint64_t* bar, uint32_t parity
   while (true) {
     if (mbar_try_wait_cluster(a, parity)) return true;
     if ((++spins & 255u) == 0u) {
-      if (*reinterpret_cast<volatile int*>(status) != 0) return false;
+      if (wait_failed(status)) return false;
       if (globaltimer() - t0 > TT_WAIT_TIMEOUT_NS) {
-        atomicCAS(status, 0, code);
+        record_failed_wait(status, code);
         return false;
       }
     }

@@ -845,8 +845,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
         if (lane == 0) {
           const uint64_t t0 = globaltimer();
           while (ld_acquire_gpu_s32(p.splitk_flags + tile) < 16 * split) {
-            if (globaltimer() - t0 > TT_WAIT_TIMEOUT_NS || *reinterpret_cast<volatile int*>(p.status) != 0) {
-              atomicCAS(p.status, 0, static_cast<int>(kTimeoutOther));
+            if (globaltimer() - t0 > TT_WAIT_TIMEOUT_NS || wait_failed(p.status)) {
+              record_failed_wait(p.status, kTimeoutOther);
               ready = false;
               break;
             }

@@ -67,9 +67,9 @@ __device__ __forceinline__ bool wait_peers(const PeerTable& t, uint64_t e, int* 
     if (p == t.rank) continue;
     const uint64_t* f = flag_ptr(t, t.rank, p);
     while (ld_acquire_sys_u64(f) < e) {
-      if (status != nullptr && *reinterpret_cast<volatile int*>(status) != 0) return false;
+      if (status != nullptr && wait_failed(status)) return false;
       if (globaltimer() - t0 > timeout_ns) {
-        if (status != nullptr) atomicCAS(status, 0, static_cast<int>(kTimeoutPeer));
+        if (status != nullptr) record_failed_wait(status, kTimeoutPeer);
         return false;
       }
       __nanosleep(64);

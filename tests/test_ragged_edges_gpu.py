@@ -279,3 +279,18 @@ def test_rotary_append_gives_zeros_at_bad_positions_and_the_rest_right():
         if where is not None:
             kw[where], vw[where] = k[i], qkv[i].view(-1, d)[hq + hkv:]
     assert torch.equal(kp, kw) and torch.equal(vp, vw)
+
+
+def test_a_recorded_bad_index_does_not_stop_later_kernels():
+    """An index out of range costs its own entry only: kernels that run before the host looks are whole."""
+    lens = [3000, 500, 45]
+    q, k, v, do = packed_inputs(lens, 8, 2, 128, seed=6)
+    clean = run_packed(q, k, v, do, cu_of(lens))
+    a, b = randn(gen(7), 4096, 2048), randn(gen(8), 2048, 2048)
+    prod = ops().linear(a, b)
+    assert status_and_clear() == 0
+    ops().token_stats(torch.zeros(1, 8, device=DEV), torch.tensor([8], device=DEV))
+    got = run_packed(q, k, v, do, cu_of(lens))
+    assert all(torch.equal(x, y) for x, y in zip(got, clean))
+    assert torch.equal(ops().linear(a, b), prod)
+    assert status_and_clear() == K_BAD_INDEX
