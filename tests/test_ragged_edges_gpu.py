@@ -294,3 +294,51 @@ def test_a_recorded_bad_index_does_not_stop_later_kernels():
     assert all(torch.equal(x, y) for x, y in zip(got, clean))
     assert torch.equal(ops().linear(a, b), prod)
     assert status_and_clear() == K_BAD_INDEX
+
+
+# ----------------------------------------------------------------------------- errors reach the caller
+def _cfg():
+    from tinytron_b200.models import ModelConfig
+
+    return ModelConfig(block_size=256, vocab_size=256, num_layer=1, num_attention_heads=4, num_key_value_heads=2, hidden_size=256,
+                       intermediate_size=256, init_std=0.05, seed=5)
+
+
+def test_ragged_generation_raises_on_a_recorded_error(monkeypatch):
+    from tinytron_b200.inference import InferenceEngine, RaggedKVCache
+
+    eng = InferenceEngine(_cfg(), device=DEV, kv_cache_page_size=16)
+    cache = RaggedKVCache.from_model_config(_cfg(), 20, 16, 4, eng.device, torch.bfloat16)
+    prompts = [torch.tensor([5, 9, 3]), torch.tensor([7])]
+    real = RaggedKVCache.prefill_step
+    with monkeypatch.context() as m:  # a prompt's page that is not mapped
+        m.setattr(RaggedKVCache, "prefill_step", lambda self, *a: (lambda s: s._replace(page_table=torch.full_like(s.page_table, -1)))(real(self, *a)))
+        with pytest.raises(RuntimeError, match="index"):
+            eng.generate_ragged(prompts, 4, cache=cache)
+    assert cache.free_pages == 20
+    out = eng.generate_ragged(prompts, 4, cache=cache)
+    assert out.lengths.tolist() == [4, 4]
+
+
+def test_launcher_does_not_step_on_a_recorded_error(monkeypatch):
+    from tinytron_b200.launch import ragged as launch
+
+    real, steps = launch.make_ragged_rollout, []
+
+    def bad(gen):
+        ro = real(gen)
+        ro.cu_seqlens = ro.cu_seqlens + torch.tensor([0] * (ro.cu_seqlens.numel() - 1) + [5], dtype=torch.int32, device=DEV)
+        return ro
+
+    class Sgd(torch.optim.AdamW):
+        def step(self, *a, **k):
+            steps.append(1)
+            return super().step(*a, **k)
+
+    monkeypatch.setattr(launch, "make_ragged_rollout", bad)
+    monkeypatch.setattr(torch.optim, "AdamW", Sgd)
+    with pytest.raises(RuntimeError, match="index"):
+        launch.main(["--device", "cuda", "--num_layer", "1", "--hidden_size", "256", "--num_attention_heads", "4",
+                     "--num_key_value_heads", "2", "--intermediate_size", "256", "--vocab_size", "256", "--block_size", "256",
+                     "--prompt_len", "2", "40", "--max_new_tokens", "4", "--num_prompts", "2", "--num_samples", "2", "--steps", "1"])
+    assert not steps

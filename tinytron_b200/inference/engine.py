@@ -180,7 +180,7 @@ class InferenceEngine:
         then on.  Returns a :class:`~tinytron_b200.inference.ragged.RaggedGeneration` with the tokens, the log-prob
         each was drawn with, the model's own log-prob and entropy, and ``alternatives`` top tokens per step.
         ``cache``: a :class:`~tinytron_b200.inference.ragged.RaggedKVCache` to work in (default: one of the right
-        size for this call); the sequences are freed again.  SEP size must be 1."""
+        size for this call); the sequences are freed again.  Raises if a kernel recorded an error.  SEP size must be 1."""
         from .ragged import generate_ragged
 
         return generate_ragged(self, prompts, max_new_tokens, num_samples, temperature, top_k, top_p, eos_token_id,

@@ -390,10 +390,12 @@ def generate_ragged(engine, prompts: Sequence[torch.Tensor], max_new_tokens: int
                     graph.replay()
                 else:
                     draw(advance())
-            if dev.type == "cuda":
-                torch.cuda.synchronize()  # before the graph's memory goes
+        if dev.type == "cuda":
+            torch.cuda.synchronize()  # before the graph's memory goes
     finally:
         cache.free([s for s in seqs if cache._rows[s] is not None])
+    if dev.type == "cuda":
+        ops.check_status(dev)  # a skipped entry or a failed wait: the tokens are not to be used
     steps = int(draw.rng[1].item())
     lengths = torch.full((n,), steps, dtype=torch.long, device=dev)
     if eos_token_id is not None:

@@ -14,6 +14,7 @@ import time
 
 import torch
 
+from tinytron_b200 import ops
 from tinytron_b200.inference import InferenceEngine
 from tinytron_b200.models import GPT
 from tinytron_b200.models.config import add_model_config_args, build_model_config
@@ -68,6 +69,8 @@ def main(argv: list[str] | None = None) -> list[dict]:
                                temperature=args.temperature)
         optim.zero_grad(set_to_none=True)
         out.loss.backward()
+        if engine.device.type == "cuda":
+            ops.check_status(engine.device)  # no step on gradients of skipped entries
         optim.step()
         loss = float(out.loss.detach())
         t2 = time.perf_counter()

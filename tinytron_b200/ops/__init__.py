@@ -23,16 +23,23 @@ def _cuda_fn():
     return functional
 
 
+_SMEM_TOO_SMALL, _BAD_INDEX = 7, 8  # StatusCode of csrc/common/ptx.cuh
+
+
 def check_status(device=None, clear: bool = True) -> int:
-    """Read the device status word written by bounded device-side waits; raise on error."""
+    """Read the device status word, which kernels set when a bounded wait ran out or an index input was out of range;
+    raise on either."""
     from . import _ext
 
-    dev = torch.cuda.current_device() if device is None else torch.device(device).index or 0
+    index = None if device is None else torch.device(device).index
+    dev = torch.cuda.current_device() if index is None else index
     code = int(_ext.load().status_read(dev))
     if code != 0:
         if clear:
             _ext.load().status_clear(dev)
-        raise RuntimeError(f"tinytron_b200 device wait timed out (status code {code}) on cuda:{dev}")
+        what = {_SMEM_TOO_SMALL: "shared memory was too small for a kernel",
+                _BAD_INDEX: "an index input was out of range (offsets, position, page, token or column); its entry was skipped"}
+        raise RuntimeError(f"tinytron_b200 {what.get(code, 'device wait timed out')} (status code {code}) on cuda:{dev}")
     return code
 
 

@@ -53,7 +53,8 @@ def make_ragged_rollout(generation, ignore_index: int = -100) -> RaggedRollout:
 def ragged_grpo_loss(model, rollout: RaggedRollout, advantages: torch.Tensor, clip_range: float = 0.2,
                      entropy_coef: float = 0.0, temperature: float = 1.0) -> RLLossOutput:
     """GRPO objective of the packed answers (``advantages`` [S], one per sequence), less ``entropy_coef`` times the
-    mean entropy of the scored positions; metrics also carry that mean."""
+    mean entropy of the scored positions; metrics also carry that mean.  On CUDA, offsets or labels out of range are found
+    on the device: call ``ops.check_status()`` before stepping on the gradients."""
     if tuple(advantages.shape) != (rollout.cu_seqlens.numel() - 1,):
         raise ValueError(f"advantages must have one entry per sequence ({rollout.cu_seqlens.numel() - 1}), got {tuple(advantages.shape)}")
     stats = model.packed_token_stats(rollout.tokens, rollout.labels, rollout.cu_seqlens, max_seqlen=rollout.max_seqlen,
