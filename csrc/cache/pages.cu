@@ -200,6 +200,7 @@ __device__ __forceinline__ void copy_page_piece(const CopyArgs& a, long long blk
 
 // Child c_i takes the row and length of parent p_i; where fresh f_i >= 0, the parent's page that
 // its next token falls into (the partly filled one) is copied to f_i and replaced by it in the child's row.
+// The blocks of an entry's data and the one of its row make the same test: an entry is done whole or not at all.
 __global__ void __launch_bounds__(kThreads) fork_kernel(const CopyArgs a) {
   const long long blk = blockIdx.x;
   const bool data = blk < a.data_blocks;
@@ -211,24 +212,39 @@ __global__ void __launch_bounds__(kThreads) fork_kernel(const CopyArgs a) {
   }
   const int len = a.lens[parent];
   const int last = len / a.page_size;
-  if (len < 0 || (fresh >= 0 && last >= a.width)) {
+  int src = -1;  // the page that is copied
+  if (len >= 0 && fresh >= 0 && last < a.width) src = a.table[static_cast<long long>(parent) * a.width + last];
+  if (len < 0 || (fresh >= 0 && (src < 0 || src >= a.num_pages || src == fresh))) {
     bad_index(a.status);
     return;
   }
   if (data) {
-    if (fresh < 0) return;
-    const int src = a.table[static_cast<long long>(parent) * a.width + last];
-    if (src < 0 || src >= a.num_pages || src == fresh) {
-      bad_index(a.status);
-      return;
-    }
-    copy_page_piece<false>(a, blk, src, fresh);
+    if (fresh >= 0) copy_page_piece<false>(a, blk, src, fresh);
     return;
   }
   const int* from = a.table + static_cast<long long>(parent) * a.width;
   int* to = a.table + static_cast<long long>(child) * a.width;
   for (int j = threadIdx.x; j < a.width; j += kThreads) to[j] = (fresh >= 0 && j == last) ? fresh : from[j];
   if (threadIdx.x == 0) a.lens[child] = len;
+}
+
+// Entry i of a move is taken where bisection for src_i over the sources ends at i.  The table's blocks look their pages
+// up by that bisection, so data and table agree on every entry, in order or not; and of two neighbours that do not
+// ascend one at least fails (the search for the second passes the first).  The probes on the way to a known index need
+// no waiting for each other: lane s checks the one of step s.
+__device__ __forceinline__ bool found_at(const int* sorted, int n, int i, int key) {
+  const int lane = threadIdx.x & 31;
+  int lo = 0, hi = n;
+  for (int s = 0; s < lane && lo < hi; ++s) {
+    const int mid = (lo + hi) >> 1;
+    if (mid < i) lo = mid + 1;
+    else hi = mid;
+  }
+  const int mid = (lo + hi) >> 1;
+  return __all_sync(0xffffffffu, lo >= hi || (sorted[mid] < key) == (mid < i));
+}
+__device__ __forceinline__ bool movable(int src, int dst, int num_pages) {
+  return src >= 0 && src < num_pages && dst >= 0 && dst < num_pages && src != dst;
 }
 
 // Page src_i becomes dst_i (src ascending, dst a free page): data of every layer, and every
@@ -238,7 +254,7 @@ __global__ void __launch_bounds__(kThreads) move_kernel(const CopyArgs a) {
   if (blk < a.data_blocks) {
     const int i = static_cast<int>(blk / (static_cast<long long>(a.chunks) * 2 * a.layers));
     const int src = a.a0[i], dst = a.a1[i];
-    if (src < 0 || src >= a.num_pages || dst < 0 || dst >= a.num_pages || src == dst || (i > 0 && a.a0[i - 1] >= src)) {
+    if (!found_at(a.a0, a.n, i, src) || !movable(src, dst, a.num_pages)) {
       bad_index(a.status);
       return;
     }
@@ -257,7 +273,7 @@ __global__ void __launch_bounds__(kThreads) move_kernel(const CopyArgs a) {
   }
   if (lo < a.n && a.a0[lo] == page) {
     const int dst = a.a1[lo];
-    if (dst >= 0 && dst < a.num_pages) a.table[e] = dst;
+    if (movable(page, dst, a.num_pages)) a.table[e] = dst;
   }
 }
 

@@ -12,6 +12,10 @@ from tinytron_b200.models import GPT, ModelConfig
 from tinytron_b200.rl import group_advantages, make_ragged_rollout, ragged_grpo_loss
 
 
+def i32(x):
+    return torch.tensor(x, dtype=torch.int32)
+
+
 # ----------------------------------------------------------------------------- token statistics
 def test_token_stats_ids_follow_the_logits():
     """Logits that differ by less than a log-prob's rounding are in their own order; a NaN is below every number."""
@@ -69,3 +73,17 @@ def cfg(**kw):
                 intermediate_size=96, init_std=0.05, seed=3)
     base.update(kw)
     return ModelConfig(**base)
+
+
+def test_fork_and_move_refuse_bad_entries_and_change_nothing():
+    g = torch.Generator().manual_seed(2)
+    kp, vp = torch.randn(2, 8, 4, 1, 8, generator=g), torch.randn(2, 8, 4, 1, 8, generator=g)
+    table, n = i32([[0, 1, 5], [-1, -1, -1], [2, -1, -1], [-1, -1, -1]]), i32([6, 0, 4, 0])
+    was = [x.clone() for x in (kp, vp, table, n)]
+    for par, kid, new in ((5, 1, 3), (0, 7, 3), (0, 0, 3), (0, 1, 8), (-1, 1, 3), (2, 1, 3), (0, 1, 1)):
+        with pytest.raises(ValueError):
+            ops.fork_pages(kp, vp, table, n, i32([0, par]), i32([3, kid]), i32([6, new]))
+    for src, dst in (([8], [3]), ([5], [-1]), ([5], [8]), ([5, 2], [3, 4]), ([2, 2], [3, 4]), ([5], [5]), ([-1], [3])):
+        with pytest.raises(ValueError):
+            ops.move_pages(kp, vp, table, i32(src), i32(dst))
+    assert all(torch.equal(a, b) for a, b in zip((kp, vp, table, n), was))

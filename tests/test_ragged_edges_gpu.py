@@ -342,3 +342,44 @@ def test_launcher_does_not_step_on_a_recorded_error(monkeypatch):
                      "--num_key_value_heads", "2", "--intermediate_size", "256", "--vocab_size", "256", "--block_size", "256",
                      "--prompt_len", "2", "40", "--max_new_tokens", "4", "--num_prompts", "2", "--num_samples", "2", "--steps", "1"])
     assert not steps
+
+
+# ----------------------------------------------------------------------------- fork and move
+def test_fork_and_move_leave_rejected_entries_alone():
+    g = gen(14)
+    kp, vp = randn(g, 2, 8, 4, 1, 8), randn(g, 2, 8, 4, 1, 8)
+    table, n = i32([[0, 1, 5], [-1, -1, -1], [2, -1, -1], [-1, -1, -1], [-1, -1, -1]]), i32([6, 0, 4, 0, 0])
+
+    def after(f):
+        x = [y.clone() for y in (kp, vp, table, n)]
+        f(*x)
+        assert status_and_clear() == K_BAD_INDEX
+        return x
+
+    def same(got, want=(kp, vp, table, n)):
+        return all(torch.equal(a, b) for a, b in zip(got, want))
+
+    for par, kid, new in ((5, 1, 3), (0, 7, 3), (0, 0, 3), (0, 1, 8), (-1, 1, 3), (2, 1, 3), (0, 1, 1)):
+        got = after(lambda k, v, t, s: ops().fork_pages(k, v, t, s, i32([par]), i32([kid]), i32([new])))
+        assert same(got), (par, kid, new)
+        # beside a good entry, which is done
+        want = [y.clone() for y in (kp, vp, table, n)]
+        ops().fork_pages(*want, i32([0]), i32([4]), i32([6]))
+        got = after(lambda k, v, t, s: ops().fork_pages(k, v, t, s, i32([par, 0]), i32([kid, 4]), i32([new, 6])))
+        assert same(got, want), (par, kid, new)
+    for src, dst in (([8], [3]), ([5], [-1]), ([5], [8]), ([5, 2], [3, 4]), ([2, 2], [3, 4]), ([5], [5]), ([-1], [3])):
+        got = after(lambda k, v, t, s: ops().move_pages(k, v, t, i32(src), i32(dst)))
+        if src == [2, 2]:  # the first is taken, the second is not ascending
+            want = [y.clone() for y in (kp, vp, table, n)]
+            ops().move_pages(*want[:3], i32([2]), i32([3]))
+            assert same(got, want)
+        else:
+            assert same([x for x in got]), (src, dst)
+    # the entries that are in order among some that are not: data and table agree
+    src, dst = [0, 5, 1, 2], [3, 4, 6, 7]
+    k, v, t, s = after(lambda k, v, t, s: ops().move_pages(k, v, t, i32(src), i32(dst)))
+    for old, new in zip(src, dst):
+        moved = bool((t == new).any())
+        assert bool((t == old).any()) != moved
+        for x, x0 in ((k, kp), (v, vp)):
+            assert torch.equal(x[:, new], x0[:, old] if moved else x0[:, new])

@@ -299,6 +299,14 @@ def fork_pages(k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.T
         return
     page = k_pages.shape[-3]
     kp, vp = (x if x.dim() == 5 else x.unsqueeze(0) for x in (k_pages, v_pages))
+    rows, width = page_table.shape
+    for par, kid, new in zip(parents.tolist(), children.tolist(), fresh.tolist()):
+        if not (0 <= par < rows and 0 <= kid < rows) or par == kid or new >= kp.shape[1]:
+            raise ValueError(f"parent {par}, child {kid} or page {new} is out of range")
+        last = int(seq_lens[par]) // page
+        old = int(page_table[par, last]) if new >= 0 and 0 <= last < width else -1
+        if last < 0 or new >= 0 and (not 0 <= old < kp.shape[1] or old == new):
+            raise ValueError(f"sequence {par} has no page to copy to {new}")
     for par, kid, new in zip(parents.tolist(), children.tolist(), fresh.tolist()):
         page_table[kid] = page_table[par]
         seq_lens[kid] = seq_lens[par]
@@ -326,6 +334,8 @@ def move_pages(k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.T
         return
     kp, vp = (x if x.dim() == 5 else x.unsqueeze(0) for x in (k_pages, v_pages))
     s, t = src.long(), dst.long()
+    if bool(((s < 0) | (s >= kp.shape[1]) | (t < 0) | (t >= kp.shape[1]) | (s == t)).any()) or bool((s[1:] <= s[:-1]).any()):
+        raise ValueError("src must ascend, and src and dst be different pages of the pool")
     kp[:, t] = kp[:, s]
     vp[:, t] = vp[:, s]
     to = torch.arange(kp.shape[1], dtype=torch.int32)
