@@ -7,7 +7,7 @@ import torch
 
 import ragged_oracle as oracle
 from tinytron_b200 import ops
-from tinytron_b200.inference import InferenceEngine
+from tinytron_b200.inference import InferenceEngine, RaggedKVCache
 from tinytron_b200.models import GPT, ModelConfig
 from tinytron_b200.rl import group_advantages, make_ragged_rollout, ragged_grpo_loss
 
@@ -87,3 +87,32 @@ def test_fork_and_move_refuse_bad_entries_and_change_nothing():
         with pytest.raises(ValueError):
             ops.move_pages(kp, vp, table, i32(src), i32(dst))
     assert all(torch.equal(a, b) for a, b in zip((kp, vp, table, n), was))
+
+
+# ----------------------------------------------------------------------------- the cache after an error
+def state(cache):
+    return (list(map(lambda r: None if r is None else list(r), cache._rows)), list(cache._lens), list(cache._refs),
+            sorted(cache._free), sorted(cache._free_seqs))
+
+
+def test_fork_that_fails_gives_back_what_it_took(monkeypatch):
+    cache = RaggedKVCache(1, 1, 2, 10, 4, 6, 16, "cpu", torch.float32)
+    a, b = cache.add(2)
+    cache.reserve([a, b], [6, 4])
+    cache.advance([a, b], [6, 4])
+    before = state(cache)
+
+    def fail(*_):
+        raise RuntimeError("no launch")
+
+    with monkeypatch.context() as m:
+        m.setattr(ops, "fork_pages", fail)
+        with pytest.raises(RuntimeError, match="no launch"):
+            cache.fork([a, a, b])
+    assert state(cache) == before
+    kids = cache.fork([a, a, b])  # and it works afterwards
+    cache._sync()
+    assert [cache.length(k) for k in kids] == [6, 6, 4]
+    assert cache.page_table[kids[0]].tolist()[0] == cache.pages_of(a)[0]
+    cache.free([a, b, *kids])
+    assert cache.free_pages == 10

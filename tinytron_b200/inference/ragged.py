@@ -151,9 +151,15 @@ class RaggedKVCache:
             raise RuntimeError("KV cache page pool or sequence table exhausted")
         kids = self.add(len(parents))
         fresh = [self._take(1)[0] if x else -1 for x in part]
-        self._sync()
-        i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=self.device)  # noqa: E731
-        ops.fork_pages(self.k_pages, self.v_pages, self.page_table, self.seq_lens, i32(list(parents)), i32(kids), i32(fresh))
+        try:
+            self._sync()
+            i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=self.device)  # noqa: E731
+            ops.fork_pages(self.k_pages, self.v_pages, self.page_table, self.seq_lens, i32(list(parents)), i32(kids), i32(fresh))
+        except BaseException:  # nothing was forked: what was taken goes back
+            for c, f in zip(kids, fresh):
+                self._rows[c] = [f] if f >= 0 else []
+            self.free(kids)
+            raise
         for p, c, f in zip(parents, kids, fresh):
             full = self._lens[p] // self.page_size
             self._rows[c] = self._rows[p][:full] + ([f] if f >= 0 else [])
