@@ -116,3 +116,21 @@ def test_fork_that_fails_gives_back_what_it_took(monkeypatch):
     assert cache.page_table[kids[0]].tolist()[0] == cache.pages_of(a)[0]
     cache.free([a, b, *kids])
     assert cache.free_pages == 10
+
+
+# ----------------------------------------------------------------------------- the policy loss
+def test_ignore_index_of_a_rollout_is_the_losss():
+    c = cfg()
+    eng = InferenceEngine(c, device="cpu", dtype=torch.float32, kv_cache_page_size=4)
+    torch.manual_seed(0)
+    gen = eng.generate_ragged([torch.tensor([3, 4, 5]), torch.tensor([6])], 5, num_samples=3)
+    actor = GPT(c, device="cpu")
+    actor.load_state_dict(eng.model.state_dict())
+    adv = group_advantages(torch.arange(6.0), 3)
+    outs = []
+    for ignore in (-100, -7):
+        ro = make_ragged_rollout(gen, ignore_index=ignore)
+        assert int((ro.labels == ignore).sum()) == ro.labels.numel() - int(gen.lengths.sum())
+        outs.append(ragged_grpo_loss(actor, ro, adv, entropy_coef=0.1))
+    assert torch.equal(outs[0].loss, outs[1].loss)
+    assert abs(float(outs[1].metrics["mean_ratio"]) - 1) < 1e-4

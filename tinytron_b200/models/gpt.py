@@ -165,10 +165,10 @@ class GPT(nn.Module):
             targets.shape)
 
     def packed_token_stats(self, idx, targets, cu_seqlens, top_k: int = 0, max_seqlen: int | None = None,
-                           temperature: float = 1.0):
+                           temperature: float = 1.0, ignore_index: int | None = None):
         """Statistics (:class:`~tinytron_b200.ops.TokenStats`, differentiable) of ``targets`` [N] under the model's
         next-token distributions at ``temperature`` over sequences packed end to end: ``idx`` [N], ``cu_seqlens`` int32 [S + 1].
-        Targets equal to the ignore index (-100) are not scored."""
+        Targets equal to ``ignore_index`` (default: the training loss's, -100) are not scored."""
         x = ops.embedding(idx, self.wte.weight)
         pending = None
         for blk in self.blocks:
@@ -179,7 +179,8 @@ class GPT(nn.Module):
             pending = (out[0] if self.use_moe else out).squeeze(0)
         _, h = ops.add_rmsnorm(x, pending, self.lnf.weight, self.eps)
         logits = ops.linear(h, self.lm_head.weight)
-        return ops.token_stats(logits, targets, top_k, self.loss_fn.ignore_index, temperature)
+        return ops.token_stats(logits, targets, top_k, self.loss_fn.ignore_index if ignore_index is None else ignore_index,
+                               temperature)
 
     @torch.no_grad()
     def forward_ragged(self, idx, step, rows=None):

@@ -19,8 +19,8 @@ from .types import RLLossOutput
 @dataclass
 class RaggedRollout:
     """Sequences packed end to end: ``tokens`` [N], ``cu_seqlens`` int32 [S + 1]; ``labels`` [N] is the next token
-    where it belongs to the answer (-100 elsewhere), ``old_log_probs`` [N] the sampler's log-prob of that token,
-    ``sequence`` [N] the row's sequence."""
+    where it belongs to the answer (``ignore_index`` elsewhere), ``old_log_probs`` [N] the sampler's log-prob of that
+    token, ``sequence`` [N] the row's sequence."""
 
     tokens: torch.Tensor
     cu_seqlens: torch.Tensor
@@ -28,6 +28,7 @@ class RaggedRollout:
     old_log_probs: torch.Tensor
     sequence: torch.Tensor
     max_seqlen: int
+    ignore_index: int = -100
 
 
 def make_ragged_rollout(generation, ignore_index: int = -100) -> RaggedRollout:
@@ -47,7 +48,7 @@ def make_ragged_rollout(generation, ignore_index: int = -100) -> RaggedRollout:
     total = [s.numel() for s in seqs]
     cu = torch.tensor([0, *total], dtype=torch.int32).cumsum(0, dtype=torch.int32).to(dev)
     owner = torch.arange(len(seqs), device=dev).repeat_interleave(torch.tensor(total, device=dev))
-    return RaggedRollout(torch.cat(seqs), cu, torch.cat(labels), torch.cat(old), owner, max(total))
+    return RaggedRollout(torch.cat(seqs), cu, torch.cat(labels), torch.cat(old), owner, max(total), ignore_index)
 
 
 def ragged_grpo_loss(model, rollout: RaggedRollout, advantages: torch.Tensor, clip_range: float = 0.2,
@@ -58,8 +59,8 @@ def ragged_grpo_loss(model, rollout: RaggedRollout, advantages: torch.Tensor, cl
     if tuple(advantages.shape) != (rollout.cu_seqlens.numel() - 1,):
         raise ValueError(f"advantages must have one entry per sequence ({rollout.cu_seqlens.numel() - 1}), got {tuple(advantages.shape)}")
     stats = model.packed_token_stats(rollout.tokens, rollout.labels, rollout.cu_seqlens, max_seqlen=rollout.max_seqlen,
-                                     temperature=temperature)
-    mask = rollout.labels.ne(-100).to(torch.float32)
+                                     temperature=temperature, ignore_index=rollout.ignore_index)
+    mask = rollout.labels.ne(rollout.ignore_index).to(torch.float32)
     adv = advantages.to(stats.log_probs.dtype)[rollout.sequence]
     out = grpo_loss(stats.log_probs, rollout.old_log_probs, adv, mask, clip_range=clip_range)
     entropy = (stats.entropy * mask).sum() / mask.sum().clamp_min(1.0)
