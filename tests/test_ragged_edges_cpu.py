@@ -75,6 +75,16 @@ def cfg(**kw):
     return ModelConfig(**base)
 
 
+@pytest.mark.parametrize("cu", [[0, 11], [1, 10], [0, 7, 5, 10], [0, -2, 10]], ids=str)
+def test_packed_attention_refuses_bad_offsets(cu):
+    g = torch.Generator().manual_seed(0)
+    q, k, v = (torch.randn(10, h, 16, generator=g) for h in (4, 2, 2))
+    with pytest.raises(ValueError, match="cu_seqlens"):
+        ops.packed_attention(q, k, v, i32(cu))
+    with pytest.raises(ValueError, match="cu_seqlens"):
+        ops.packed_attention(q, k, v, i32([0] + [10] * (len(cu) - 1)), i32(cu))
+
+
 def test_fork_and_move_refuse_bad_entries_and_change_nothing():
     g = torch.Generator().manual_seed(2)
     kp, vp = torch.randn(2, 8, 4, 1, 8, generator=g), torch.randn(2, 8, 4, 1, 8, generator=g)

@@ -62,10 +62,18 @@ def _kernel_rows(t: torch.Tensor) -> torch.Tensor:
 
 
 # ----------------------------------------------------------------------------- packed attention
+def _offsets_cpu(name: str, cu: torch.Tensor, tokens: int) -> list[int]:
+    """The offsets as numbers; on CUDA the kernels make the same test."""
+    c = cu.tolist()
+    if c[0] != 0 or c[-1] > tokens or any(b < a for a, b in zip(c, c[1:])):
+        raise ValueError(f"{name} must ascend from 0 to at most {tokens}, got {c}")
+    return c
+
+
 def _packed_attention_cpu(q, k, v, cu_q, cu_k, scale):
     g = q.shape[1] // k.shape[1]
     out = []
-    cq, ck = cu_q.tolist(), cu_k.tolist()
+    cq, ck = _offsets_cpu("cu_seqlens", cu_q, q.shape[0]), _offsets_cpu("cu_seqlens_k", cu_k, k.shape[0])
     for b in range(len(cq) - 1):
         n, m = cq[b + 1] - cq[b], ck[b + 1] - ck[b]
         qs = q[cq[b]:cq[b + 1]].float().transpose(0, 1)
@@ -132,7 +140,7 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
 
     q [Nq, Hq, D], k/v [Nk, Hkv, D] bf16, D 64 or 128, Hq a multiple of Hkv, any strides with contiguous
     16-byte-aligned head rows (slices of one packed projection are read in place).  ``cu_seqlens``
-    int32 [B + 1] on the same device: sequence b is rows [cu[b], cu[b + 1]) (lengths of zero are
+    int32 [B + 1] on the same device, ascending from 0: sequence b is rows [cu[b], cu[b + 1]) (lengths of zero are
     allowed).  ``cu_seqlens_k`` gives the keys' rows where they differ: the sequences then end together,
     query i sees keys j <= i + (len_k - len_q).  Queries that see no key, and rows after the last
     sequence, get zeros (and zero gradients).  Returns o [Nq, Hq, D]; differentiable in q, k and v."""
