@@ -85,6 +85,21 @@ def test_packed_attention_refuses_bad_offsets(cu):
         ops.packed_attention(q, k, v, i32([0] + [10] * (len(cu) - 1)), i32(cu))
 
 
+def test_rotary_append_tokens_before_the_first_sequence_belong_to_none():
+    from tinytron_b200.ops.rope import rope_tables
+
+    g = torch.Generator().manual_seed(1)
+    qkv = torch.randn(7, 8 * 8, generator=g)
+    cos, sin = rope_tables(8, 10000.0, 64, "cpu")
+    kp, vp = torch.zeros(3, 4, 2, 8), torch.zeros(3, 4, 2, 8)
+    q, k = ops.rotary_append(qkv, cos, sin, 4, 2, i32([2, 5]), None, kp, vp, i32([[1]]))
+    want = ops.rotary_append(qkv[2:5], cos, sin, 4, 2, i32([0, 3]))
+    assert torch.equal(q[2:5], want[0]) and torch.equal(k[2:5], want[1])
+    for x in (q, k):
+        assert bool((x[:2] == 0).all()) and bool((x[5:] == 0).all())
+    assert bool((kp[0] == 0).all()) and bool((kp[2] == 0).all()) and torch.equal(kp[1, :3], want[1])
+
+
 def test_fork_and_move_refuse_bad_entries_and_change_nothing():
     g = torch.Generator().manual_seed(2)
     kp, vp = torch.randn(2, 8, 4, 1, 8, generator=g), torch.randn(2, 8, 4, 1, 8, generator=g)

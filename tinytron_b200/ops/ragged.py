@@ -258,7 +258,7 @@ def rotary_append(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, num_h
     x = qkv[:, :(num_heads + 2 * num_kv_heads) * d].reshape(n, num_heads + 2 * num_kv_heads, d)
     c = cu.long()
     owner = torch.bucketize(torch.arange(n), c[1:], right=True)
-    inside = owner < cu.numel() - 1
+    inside = (owner < cu.numel() - 1) & (torch.arange(n) >= c[0])  # tokens of no sequence: before the first, after the last
     b = owner.clamp(max=max(0, cu.numel() - 2))
     if cu.numel() == 1:
         inside = torch.zeros(n, dtype=torch.bool)
