@@ -143,6 +143,27 @@ def test_fork_that_fails_gives_back_what_it_took(monkeypatch):
     assert cache.free_pages == 10
 
 
+def test_resize_that_runs_out_of_memory_changes_nothing(monkeypatch):
+    cache = RaggedKVCache(1, 1, 2, 10, 4, 6, 16, "cpu", torch.float32)
+    real, calls = torch.empty, []
+
+    def empty(*a, **k):
+        calls.append(1)
+        if len(calls) == 2:
+            raise RuntimeError("out of memory")
+        return real(*a, **k)
+
+    with monkeypatch.context() as m:
+        m.setattr(torch, "empty", empty)
+        with pytest.raises(RuntimeError, match="out of memory"):
+            cache.resize(5)
+    assert cache.k_pages.shape == cache.v_pages.shape and cache.num_pages == len(cache._refs) == 10
+    cache.resize(5)
+    assert cache.k_pages.shape[1] == cache.v_pages.shape[1] == 5 and cache.free_pages == 5
+    with pytest.raises(ValueError):
+        cache.resize(-1)
+
+
 # ----------------------------------------------------------------------------- the policy loss
 def test_ignore_index_of_a_rollout_is_the_losss():
     c = cfg()

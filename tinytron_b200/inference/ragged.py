@@ -202,14 +202,17 @@ class RaggedKVCache:
 
     def resize(self, num_pages: int) -> None:
         """A pool of another size (after :meth:`compact`, at least the pages in use)."""
+        if num_pages < 0:
+            raise ValueError(f"num_pages must not be negative, got {num_pages}")
         if any(self._refs[num_pages:]):
             raise ValueError(f"pages past {num_pages} are in use: compact() first")
         keep = min(num_pages, self.num_pages)
-        for name in ("k_pages", "v_pages"):
-            old = getattr(self, name)
+        pools = []
+        for old in (self.k_pages, self.v_pages):
             new = torch.empty((old.shape[0], num_pages, *old.shape[2:]), dtype=old.dtype, device=old.device)
             new[:, :keep] = old[:, :keep]
-            setattr(self, name, new)
+            pools.append(new)
+        self.k_pages, self.v_pages = pools  # both or, where there is no room for the second, neither
         self._refs = self._refs[:num_pages] + [0] * (num_pages - len(self._refs))
         self._free = [p for p in range(num_pages) if not self._refs[p]]
 
