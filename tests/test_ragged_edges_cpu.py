@@ -164,6 +164,26 @@ def test_resize_that_runs_out_of_memory_changes_nothing(monkeypatch):
         cache.resize(-1)
 
 
+def test_decode_step_needs_its_pages():
+    """A step whose token has no mapped page, or that names a sequence twice, is refused on the host."""
+    cache = RaggedKVCache(1, 1, 2, 10, 4, 6, 8, "cpu", torch.float32)
+    a, b = cache.add(2)
+    cache.reserve([a, b], [4, 3])
+    cache.advance([a, b], [4, 3])
+    with pytest.raises(ValueError, match="reserve"):
+        cache.decode_step([a, b])
+    with pytest.raises(ValueError, match="twice"):
+        cache.decode_step([b, b])
+    cache.reserve([a], [1])
+    step = cache.decode_step([a, b])
+    assert step.seq_lens.tolist() == [5, 4]
+    for f in (cache.reserve, cache.advance):
+        with pytest.raises(ValueError):
+            f([a], [-1])
+    with pytest.raises(ValueError):
+        cache.prefill_step([99], [2])
+
+
 # ----------------------------------------------------------------------------- the policy loss
 def test_ignore_index_of_a_rollout_is_the_losss():
     c = cfg()

@@ -119,6 +119,8 @@ class RaggedKVCache:
         self._check(*seqs)
         want = []
         for s, n in zip(seqs, tokens, strict=True):
+            if n < 0:
+                raise ValueError(f"sequence {s}: {n} tokens")
             end = self._lens[s] + n
             if end > self.max_seq_len:
                 raise ValueError(f"KV cache overflow: requested sequence length {end}, max supported is {self.max_seq_len}")
@@ -135,6 +137,8 @@ class RaggedKVCache:
         """Commit tokens whose keys and values have been written."""
         self._check(*seqs)
         for s, n in zip(seqs, tokens, strict=True):
+            if n < 0:
+                raise ValueError(f"sequence {s}: {n} tokens")
             if self._lens[s] + n > len(self._rows[s]) * self.page_size:
                 raise ValueError(f"sequence {s}: length {self._lens[s] + n} is past its mapped pages")
             self._lens[s] += n
@@ -225,6 +229,7 @@ class RaggedKVCache:
 
     def prefill_step(self, seqs: Sequence[int], tokens: Sequence[int]) -> RaggedStep:
         """A step in which ``seqs[i]``, empty so far, receives ``tokens[i]`` tokens (pages reserved here)."""
+        self._check(*seqs)
         if any(self._lens[s] for s in seqs):
             raise ValueError("prefill of a sequence that already holds tokens")
         self.reserve(seqs, tokens)
@@ -235,6 +240,12 @@ class RaggedKVCache:
     def decode_step(self, seqs: Sequence[int]) -> RaggedStep:
         """A step in which each of ``seqs`` receives one token (reserved before); ``start`` and ``seq_lens`` are
         tensors of the step's own, for a caller that replays it to advance."""
+        self._check(*seqs)
+        if len(set(seqs)) != len(seqs):
+            raise ValueError("a sequence is named twice")
+        for s in seqs:
+            if self._lens[s] >= len(self._rows[s]) * self.page_size:
+                raise ValueError(f"sequence {s}: its next position {self._lens[s]} has no page, reserve() it first")
         table, start = self._rows_of(seqs)
         cu = torch.arange(len(seqs) + 1, dtype=torch.int32, device=self.device)
         return RaggedStep(self, table, cu, start, start + 1)
