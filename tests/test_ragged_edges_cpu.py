@@ -184,6 +184,21 @@ def test_decode_step_needs_its_pages():
         cache.prefill_step([99], [2])
 
 
+def test_a_workspace_made_in_a_capture_stays_there(monkeypatch):
+    """Scratch that is cleared by a captured step holds nothing valid outside of it."""
+    cache = RaggedKVCache(1, 1, 2, 4, 4, 2, 16, "cpu", torch.float32)
+    cache.device = torch.device("cuda")
+    capturing, made = [True], []
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: capturing[0])
+    monkeypatch.setattr(ops, "paged_attention_workspace", lambda *a: made.append(object()) or made[-1])
+    inside = cache.workspace(2, 4)
+    capturing[0] = False
+    outside = cache.workspace(2, 4)
+    assert outside is not inside and cache.workspace(2, 4) is outside
+    capturing[0] = True
+    assert cache.workspace(2, 4) is outside  # cleared before the capture: shared with it
+
+
 # ----------------------------------------------------------------------------- the policy loss
 def test_ignore_index_of_a_rollout_is_the_losss():
     c = cfg()

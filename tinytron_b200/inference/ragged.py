@@ -251,14 +251,18 @@ class RaggedKVCache:
         return RaggedStep(self, table, cu, start, start + 1)
 
     def workspace(self, batch: int, num_heads: int):
-        """Decode-attention scratch for this batch, kept: the steps of one cache run one after the other."""
+        """Decode-attention scratch for this batch, kept: the steps of one cache run one after the other.  Scratch made
+        inside a capture is the capture's own: its counters are cleared by the graph's replays, not now."""
         if self.device.type != "cuda":
             return None
         key = (batch, num_heads)
-        if key not in self._workspaces:
-            self._workspaces[key] = ops.paged_attention_workspace(
-                batch, num_heads, self.k_pages.shape[3], self.k_pages.shape[4], self.width * self.page_size, self.device)
-        return self._workspaces[key]
+        if key in self._workspaces:
+            return self._workspaces[key]
+        made = ops.paged_attention_workspace(batch, num_heads, self.k_pages.shape[3], self.k_pages.shape[4],
+                                             self.width * self.page_size, self.device)
+        if not torch.cuda.is_current_stream_capturing():
+            self._workspaces[key] = made
+        return made
 
 
 @dataclass
