@@ -141,10 +141,17 @@ __global__ void __launch_bounds__(CE_THREADS) ce_fwd_kernel(__nv_bfloat16* __res
 }
 
 // ----------------------------------------------------------------- embedding
+// A token id outside the table reads nothing: zeros, and kBadIndex in the status word.
 __global__ void embedding_fwd_kernel(const int64_t* __restrict__ idx, const float* __restrict__ table,
-                                     float* __restrict__ out, int D) {
+                                     float* __restrict__ out, int D, long long V, int* status) {
   const int row = blockIdx.x;
   const int64_t t = idx[row];
+  if (t < 0 || t >= V) {
+    if (threadIdx.x == 0) atomicCAS(status, 0, static_cast<int>(kBadIndex));
+    for (int i = threadIdx.x; i < D / 4; i += blockDim.x)
+      reinterpret_cast<float4*>(out + static_cast<size_t>(row) * D)[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    return;
+  }
   const float4* src = reinterpret_cast<const float4*>(table + static_cast<size_t>(t) * D);
   float4* dst = reinterpret_cast<float4*>(out + static_cast<size_t>(row) * D);
   for (int i = threadIdx.x; i < D / 4; i += blockDim.x) dst[i] = src[i];
@@ -349,7 +356,8 @@ void embedding_fwd(torch::Tensor idx, torch::Tensor table, torch::Tensor out) {
   if (idx.numel() == 0) return;
   const c10::cuda::CUDAGuard guard(table.device());
   embedding_fwd_kernel<<<static_cast<unsigned>(idx.numel()), 256, 0, cur_stream()>>>(
-      idx.data_ptr<int64_t>(), table.data_ptr<float>(), out.data_ptr<float>(), static_cast<int>(D));
+      idx.data_ptr<int64_t>(), table.data_ptr<float>(), out.data_ptr<float>(), static_cast<int>(D), table.size(0),
+      device_status_ptr(table.get_device()));
   TT_CUDA_CHECK(cudaGetLastError());
 }
 

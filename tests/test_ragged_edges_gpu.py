@@ -320,6 +320,18 @@ def test_ragged_generation_raises_on_a_recorded_error(monkeypatch):
     assert out.lengths.tolist() == [4, 4]
 
 
+def test_a_token_outside_the_vocabulary_reads_nothing():
+    from tinytron_b200.inference import InferenceEngine
+
+    table = randn(gen(16), 50, 64, dtype=torch.float32)
+    got = ops().embedding(torch.tensor([3, -1, 49, 50, 1 << 40], device=DEV), table)
+    assert status_and_clear() == K_BAD_INDEX
+    assert torch.equal(got[[0, 2]], table[[3, 49]]) and bool((got[[1, 3, 4]] == 0).all())
+    eng = InferenceEngine(_cfg(), device=DEV, kv_cache_page_size=16)
+    with pytest.raises(RuntimeError, match="index"):
+        eng.generate_ragged([torch.tensor([5, 256]), torch.tensor([7])], 4)
+
+
 def test_launcher_does_not_step_on_a_recorded_error(monkeypatch):
     from tinytron_b200.launch import ragged as launch
 
