@@ -395,3 +395,65 @@ def test_fork_and_move_leave_rejected_entries_alone():
         assert bool((t == old).any()) != moved
         for x, x0 in ((k, kp), (v, vp)):
             assert torch.equal(x[:, new], x0[:, old] if moved else x0[:, new])
+
+
+# ----------------------------------------------------------------------------- accuracy by norms
+# A rounding to bf16 errs by ulp / sqrt(12) in the root mean square; over mantissas m spread evenly in log m that is
+# 2^-7 sqrt(E[1 / m^2] / 12) = 2^-7 sqrt(0.375 / ln 2 / 12) = 0.00166 of the value.  An output of independent terms, each with
+# one such rounding inside (P, or dS), and its own rounding: sqrt(2) of it; the short rows at a sequence's start, whose terms
+# are few, add delta's share: at most another 0.3 of its square.  With a tenth for the draw: 0.00166 sqrt(2.3) 1.1.
+ROUND = 0.00166
+NORM_BOUND = ROUND * math.sqrt(2.3) * 1.1
+
+
+def rel(got, want):
+    return float((got.double() - want).norm() / want.norm())
+
+
+@pytest.mark.parametrize("hq,hkv,d", [(8, 2, 128), (8, 2, 64), (4, 4, 128)])
+def test_packed_attention_accuracy_by_norm(hq, hkv, d):
+    lens = [700, 45, 300, 1000]
+    q, k, v, do = packed_inputs(lens, hq, hkv, d, seed=21)
+    got = run_packed(q, k, v, do, cu_of(lens))
+    ref = oracle.packed(q, k, v, cu_of(lens), do=do)
+    for x, name in zip(got, ("o", "dq", "dk", "dv")):
+        assert rel(x, ref[name]) < NORM_BOUND, (name, rel(x, ref[name]))
+
+
+@pytest.mark.parametrize("d", [64, 128])
+def test_packed_attention_keeps_what_the_outputs_rounding_left(d):
+    """o + o_lo, which delta = dO . O is taken from, carries P's rounding only; o alone has its own besides."""
+    from tinytron_b200.ops import ragged
+
+    lens = [700, 45, 300, 1000]
+    q, k, v, _ = packed_inputs(lens, 8, 2, d, seed=22)
+    cu = i32(cu_of(lens))
+    o, (o_lo, _) = ragged._packed_fwd(q, k, v, cu, cu, 1.0 / math.sqrt(d), True)
+    ref = oracle.packed(q, k, v, cu_of(lens))["o"]
+    assert rel(o.double() + o_lo.double(), ref) < ROUND * 1.1
+    assert rel(o, ref) > ROUND * 1.1  # the bound tells them apart
+
+
+def test_packed_attention_directional_derivatives():
+    """Derivatives along random directions against central differences in 64 bits, within the gradients' relative error
+    (NORM_BOUND of the gradient's norm a direction, four sigma for eight of them together); a zero and a negated gradient fail."""
+    lens, dirs, eps = [150, 9, 300], 8, 1e-5
+    q, k, v, do = packed_inputs(lens, 2, 1, 64, seed=23)
+    grads = run_packed(q, k, v, do, cu_of(lens))[1:]
+    g = gen(24)
+    for i, grad in enumerate(grads):
+        want, got = [], []
+        for _ in range(dirs):
+            base = [x.double() for x in (q, k, v)]
+            step = torch.randn(base[i].shape, generator=g, device=DEV, dtype=torch.float64)
+            f = []
+            for s in (eps, -eps):
+                x = list(base)
+                x[i] = x[i] + s * step
+                f.append(float((oracle.packed(*x, cu_of(lens))["o"] * do.double()).sum()))
+            want.append((f[0] - f[1]) / (2 * eps))
+            got.append(float((grad.double() * step).sum()))
+        want, got = torch.tensor(want, dtype=torch.float64), torch.tensor(got, dtype=torch.float64)
+        bound = 4 * NORM_BOUND * math.sqrt(dirs) * float(grad.double().norm())
+        assert float((got - want).norm()) < bound
+        assert float(want.norm()) > bound and float((got + want).norm()) > bound
