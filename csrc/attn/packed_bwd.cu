@@ -20,9 +20,14 @@
 // their rows of the operand they are multiplied with are cleared (zero times a neighbour's infinity
 // is not zero).
 //
+// P is rounded to bf16 once for dV, dS once for dQ and dK (the operands of the products); sums, delta and the
+// statistics are fp32.
+//
 // Bound by P and dS passing through TMEM between the products.  14 sequences, 16384 tokens, 16/4 heads, d 128
-// (329 GFLOP at five products): dkv 254 us, dq 211 us, the row statistics 40 us; 650 TFLOP/s in all, 910
-// counting the seven products that run.
+// (329 GFLOP at five products), each kernel by itself: dkv 257 us, dq 210 us, the row statistics 39 us; 650 TFLOP/s in
+// all, 910 counting the seven products that run; with its three schedules (14 us) and the forward the pass takes 795.  One
+// long sequence (10365 of 17001 tokens, 8/2 heads, d 64): dkv 490 us, by its longest CTA: the first key tile's column of
+// queries, all heads of the group, is 1.4 times the mean load of an SM, and an entry is not split.
 #include "attn/packed.cuh"
 #include "common/fast_exp2.cuh"
 

@@ -19,6 +19,9 @@
 // see it NaN (exp2_poly_any), as the definition does.  A NaN or infinity in V reaches the rows that see it, and may
 // reach rows of the same sequence in the same tile that do not (zero times it).
 //
+// P is rounded to bf16 once, as the A operand; its row sums take the unrounded exponentials.  Three of eight exponentials
+// are a polynomial good to 7.5e-5, a twentieth of that rounding.
+//
 // Bound by the softmax between a tile's two products (TMEM read, maxima, exponentials, P back), which the other
 // tile's products hide only in part.  14 sequences, 16384 tokens, 16/4 heads, d 128 (132 GFLOP of visible
 // pairs): 192 us, 690 TFLOP/s.  24 sequences of very different lengths (105 GFLOP): 166 us; with

@@ -20,7 +20,9 @@
 // 16; tcgen05 needs 64 and would not move one byte faster), P passing from accumulator to operand in
 // registers.  The warps' softmax states meet once per stretch, not per tile.
 //
-// Measured (L2 flushed): 140K tokens of 40/8 heads, d 128 (574 MB): 107 us, 5.4 TB/s; 32 sequences of about
+// P is rounded to bf16 once, as the MMA operand; maxima, sums, partials and the join are fp32.
+//
+// Measured (L2 flushed): 140K tokens of 40/8 heads, d 128 (574 MB): 102 us, 5.6 TB/s; 32 sequences of about
 // 1.1K tokens, 16/4 heads (74 MB): 28 us, of which about 10 are start-up and the join.
 #include "common/host_utils.h"
 #include "common/ptx.cuh"

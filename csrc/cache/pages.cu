@@ -9,9 +9,9 @@
 // Index inputs live on the device and are checked where they are used: an entry out of range is
 // skipped and recorded as kBadIndex in the status word; a token at a position past the tables comes back as zeros.
 //
-// Measured (L2 flushed): appending 16384 tokens of 16/4 heads, d 128 (218 MB): 51 us, 4.3 TB/s; moving 16 KB
-// pages of 16 layers (772 MB): 123 us, 6.3 TB/s; forking 8 prompts into 8 answers each over 16 layers
-// (537 MB counted, 302 MB of them distinct): 56 us.
+// Measured (L2 flushed): appending 16384 tokens of 16/4 heads, d 128 (218 MB): 47 us, 4.6 TB/s; moving 16 KB
+// pages of 16 layers (772 MB): 124 us, 6.2 TB/s; forking 8 prompts into 8 answers each over 16 layers
+// (537 MB counted, 302 MB of them distinct): 53 us.
 #include "common/host_utils.h"
 #include "common/ptx.cuh"
 
