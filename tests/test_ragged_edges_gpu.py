@@ -281,6 +281,29 @@ def test_rotary_append_gives_zeros_at_bad_positions_and_the_rest_right():
     assert torch.equal(kp, kw) and torch.equal(vp, vw)
 
 
+def test_bad_entries_leave_the_other_sequences_right():
+    """A page that is not mapped, a length past the table, a target outside the vocabulary: the rows beside them hold."""
+    g = gen(17)
+    q, kp, vp = randn(g, 3, 4, 64), randn(g, 9, 16, 2, 64), randn(g, 9, 16, 2, 64)
+    table, n = i32([[0, 1, 2], [3, 4, 5], [6, 7, 8]]), i32([40, 33, 48])
+    want = ops().paged_attention(q, kp, vp, table, n)
+    assert status_and_clear() == 0
+    for t, m in ((i32([[0, 1, 2], [3, -1, 5], [6, 7, 8]]), n), (i32([[0, 1, 2], [3, 99, 5], [6, 7, 8]]), n), (table, i32([40, 1000, 48])),
+                 (table, i32([40, -5, 48]))):
+        got = ops().paged_attention(q, kp, vp, t, m)
+        assert status_and_clear() == K_BAD_INDEX
+        assert torch.equal(got[0], want[0]) and torch.equal(got[2], want[2]) and bool(got.isfinite().all())
+    x = randn(g, 3, 500, dtype=torch.float32).requires_grad_(True)
+    good = ops().token_stats(x, torch.tensor([4, 7, 9], device=DEV), top_k=2)
+    (ref,) = torch.autograd.grad(good.log_probs.sum() + good.entropy.sum(), x)
+    st = ops().token_stats(x, torch.tensor([4, 500, 9], device=DEV), top_k=2)
+    (grad,) = torch.autograd.grad(st.log_probs.sum() + st.entropy.sum(), x)
+    assert status_and_clear() == K_BAD_INDEX
+    for a, b in ((st.log_probs, good.log_probs), (st.entropy, good.entropy), (st.top_ids, good.top_ids), (grad, ref)):
+        assert torch.equal(a[[0, 2]], b[[0, 2]])
+    assert bool((grad[1] == 0).all()) and float(st.log_probs[1].detach()) == 0 and st.top_ids[1].tolist() == [-1, -1]
+
+
 def test_a_recorded_bad_index_does_not_stop_later_kernels():
     """An index out of range costs its own entry only: kernels that run before the host looks are whole."""
     lens = [3000, 500, 45]
